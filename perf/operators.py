@@ -273,9 +273,9 @@ def _encode(b, signed):
 def _decode(codes, s, signed):
     c = codes.float()
     if signed:
-        return c * c.abs() * (s * (1 / 127**2))
-    c = c * c
-    return c * c * (s * (1 / 255**4))
+        return c * c.abs() * (1 / 127**2) * s
+    c = c * c * (1 / 255**2)
+    return c * c * s
 
 
 def _blocks(packed, signed):
