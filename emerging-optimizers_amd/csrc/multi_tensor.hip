@@ -1,0 +1,862 @@
+// Element-wise optimizer operators over whole lists of tensors: the AdamW step with moments in 32 or in 8 bits, the
+// global 2-norm and the scaling that clips by it, and the conversions of 8-bit moments.
+//
+// One launch serves up to a few dozen tensors.  Their addresses and sizes travel in the kernel's argument block, so a
+// call needs no table in device memory, no copy and no host wait, and a captured call replays with the addresses it was
+// captured with.  The tensors of a launch are cut into chunks that are numbered through, one workgroup a chunk; a
+// workgroup finds its tensor by bisection in the list of first chunks (uniform: scalar loads and scalar branches).
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "../../include/mi_ns.h"
+#include "launch.hpp"
+
+namespace mi {
+namespace {
+
+constexpr int NT = 256;  // threads of a workgroup
+constexpr int BLOCK8 = 64;  // values that share a scale in the 8-bit form of a moment
+// A launch's workgroup count stays below 2^24 (2^32 threads) with room to spare; one tensor must fit into one launch.
+constexpr int64_t MAX_CHUNKS = (int64_t)1 << 23;
+constexpr int64_t MAX_NUMEL = (int64_t)1 << 35;
+
+// ---------------------------------------------------------------------------------------------
+// Argument blocks (4 KB at most)
+// ---------------------------------------------------------------------------------------------
+struct AdamTensor {
+  void* p;            // weights of record, updated in place
+  const void* g;
+  void* m;            // moments: float32 values, or the 8-bit form (codes, then the blocks' scales)
+  void* v;
+  void* low;          // 16-bit copy of the updated weights, or null
+  const float* step;  // device step counter, or null (the call's own)
+  int64_t n;
+};
+struct AdamScalars {
+  float b1, omb1, b2, omb2, eps, keep, l2, step_size, inv_sqrt_bc2;
+  // for a step counter or a learning rate on the device: bias corrections and decay are evaluated by the kernel
+  int on_device, method;
+  double lr, wd, ln_b1, ln_b2, step;
+  const float* lr_dev;
+  const float* grad_scale;
+};
+template <class T, int N>
+struct TensorList {
+  static constexpr int CAPACITY = N;
+  T t[N];
+  uint32_t first[N];  // number of the tensor's first chunk
+  int count;
+};
+typedef TensorList<AdamTensor, 60> AdamList;
+struct AdamArgs {
+  AdamList list;
+  AdamScalars s;
+};
+static_assert(sizeof(AdamArgs) <= 4096, "argument block");
+
+struct ReadTensor {
+  const void* x;
+  int64_t n;
+};
+typedef TensorList<ReadTensor, 192> ReadList;
+struct MoveTensor {
+  const void* src;
+  void* dst;
+  int64_t n;
+};
+typedef TensorList<MoveTensor, 128> MoveList;
+static_assert(sizeof(ReadList) <= 4000 && sizeof(MoveList) <= 4000, "argument block");
+
+// Index of the tensor that chunk `b` belongs to: the last one whose first chunk is not behind it.
+template <class L>
+__host__ __device__ __forceinline__ int tensor_of(const L& l, uint32_t b) {
+  int lo = 0, hi = l.count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (l.first[mid] <= b) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Four values at a time.  Tensors need the alignment of their elements only: the vector types say so, and global
+// loads and stores of any width take such addresses.
+// ---------------------------------------------------------------------------------------------
+template <class T>
+struct Quad {
+  typedef T type __attribute__((ext_vector_type(4)));
+  typedef type at __attribute__((aligned(sizeof(T))));
+};
+template <class T>
+__device__ __forceinline__ f32x4_t load4(const T* p) {
+  return __builtin_convertvector((typename Quad<T>::type)(*reinterpret_cast<const typename Quad<T>::at*>(p)), f32x4_t);
+}
+template <class T>
+__device__ __forceinline__ void store4(T* p, f32x4_t x) {
+  *reinterpret_cast<typename Quad<T>::at*>(p) = __builtin_convertvector(x, typename Quad<T>::type);
+}
+// The first `k` of four values; zeros for the others.
+template <class T>
+__device__ __forceinline__ f32x4_t load4_part(const T* p, int k) {
+  f32x4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < k) x[i] = (float)p[i];
+  return x;
+}
+template <class T>
+__device__ __forceinline__ void store4_part(T* p, f32x4_t x, int k) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < k) p[i] = (T)x[i];
+}
+
+// ---------------------------------------------------------------------------------------------
+// AdamW
+// ---------------------------------------------------------------------------------------------
+struct AdamCoef {
+  float b1, omb1, b2, omb2, eps, keep, l2, step_size, inv_sqrt_bc2, gscale;
+};
+
+enum { DECAY_DECOUPLED = 0, DECAY_INDEPENDENT = 1, DECAY_L2 = 2, DECAY_PALM = 3 };
+
+// Factor of the weight and multiple of the weight that joins the gradient, by decay method.
+__host__ __device__ inline void decay_terms(int method, double wd, double lr, float* keep, float* l2) {
+  *l2 = method == DECAY_L2 ? (float)wd : 0.0f;
+  const double shrink = method == DECAY_DECOUPLED ? wd * lr : method == DECAY_INDEPENDENT ? wd : method == DECAY_PALM ? wd * lr * lr : 0.0;
+  *keep = (float)(1.0 - shrink);
+}
+// lr / (1 - b1^t) and 1 / sqrt(1 - b2^t), in 64 bits: 1 - b^t loses its leading digits for small t and b near 1.
+__host__ __device__ inline void bias_terms(double ln_b1, double ln_b2, double t, double lr, float* step_size, float* inv_sqrt_bc2) {
+  *step_size = (float)(lr / -expm1(t * ln_b1));
+  *inv_sqrt_bc2 = (float)(1.0 / sqrt(-expm1(t * ln_b2)));
+}
+
+__device__ __forceinline__ AdamCoef adam_coefficients(const AdamScalars& s, const float* step_dev) {
+  AdamCoef c = {s.b1, s.omb1, s.b2, s.omb2, s.eps, s.keep, s.l2, s.step_size, s.inv_sqrt_bc2, 1.0f};
+  if (s.on_device) {
+    const double lr = s.lr_dev ? (double)*s.lr_dev : s.lr;
+    decay_terms(s.method, s.wd, lr, &c.keep, &c.l2);
+    bias_terms(s.ln_b1, s.ln_b2, step_dev ? (double)*step_dev : s.step, lr, &c.step_size, &c.inv_sqrt_bc2);
+  }
+  if (s.grad_scale) c.gscale = *s.grad_scale;
+  return c;
+}
+
+// m <- b1 m + (1 - b1) g,  v <- b2 v + (1 - b2) g^2,  p <- keep p - step_size m / (sqrt(v) inv_sqrt_bc2 + eps)
+__device__ __forceinline__ void adam_value(float& p, float g, float& m, float& v, const AdamCoef& c) {
+  g *= c.gscale;
+  if (c.l2 != 0.0f) g = fmaf(c.l2, p, g);
+  m = fmaf(c.b1, m, c.omb1 * g);
+  v = fmaf(c.b2, v, c.omb2 * g * g);
+  const float den = fmaf(sqrtf(v), c.inv_sqrt_bc2, c.eps);
+  p = fmaf(-c.step_size, m / den, c.keep * p);
+}
+
+// 32-bit moments.  Each value is read and written once: 28 bytes a value with float32 weights and gradients, about 25
+// operations, so the memory bounds it.
+constexpr int ADAM_U = 4;
+constexpr int ADAM_CHUNK = NT * 4 * ADAM_U;
+
+struct None {};
+
+template <class PT, class GT, class LT>
+__global__ __launch_bounds__(NT) void adamw_kernel(AdamArgs a) {
+  const int ti = tensor_of(a.list, blockIdx.x);
+  const AdamTensor t = a.list.t[ti];
+  const int64_t base = (int64_t)(blockIdx.x - a.list.first[ti]) * ADAM_CHUNK;
+  PT* __restrict__ p = static_cast<PT*>(t.p) + base;
+  const GT* __restrict__ g = static_cast<const GT*>(t.g) + base;
+  float* __restrict__ m = static_cast<float*>(t.m) + base;
+  float* __restrict__ v = static_cast<float*>(t.v) + base;
+  const int64_t left = t.n - base;
+  const AdamCoef c = adam_coefficients(a.s, t.step);
+  if (left >= ADAM_CHUNK) {
+    f32x4_t pp[ADAM_U], gg[ADAM_U], mm[ADAM_U], vv[ADAM_U];
+#pragma unroll
+    for (int u = 0; u < ADAM_U; ++u) {
+      const int e = (u * NT + threadIdx.x) * 4;
+      gg[u] = load4(g + e);
+      pp[u] = load4(p + e);
+      mm[u] = load4(m + e);
+      vv[u] = load4(v + e);
+    }
+#pragma unroll
+    for (int u = 0; u < ADAM_U; ++u) {
+      const int e = (u * NT + threadIdx.x) * 4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float pi = pp[u][i], mi = mm[u][i], vi = vv[u][i];
+        adam_value(pi, gg[u][i], mi, vi, c);
+        pp[u][i] = pi;
+        mm[u][i] = mi;
+        vv[u][i] = vi;
+      }
+      store4(p + e, pp[u]);
+      store4(m + e, mm[u]);
+      store4(v + e, vv[u]);
+      if constexpr (!__is_same(LT, None)) store4(static_cast<LT*>(t.low) + base + e, pp[u]);
+    }
+    return;
+  }
+  for (int u = 0; u < ADAM_U; ++u) {
+    const int e = (u * NT + threadIdx.x) * 4;
+    if (e >= left) return;
+    const int k = left - e < 4 ? (int)(left - e) : 4;
+    f32x4_t pp = load4_part(p + e, k), gg = load4_part(g + e, k), mm = load4_part(m + e, k), vv = load4_part(v + e, k);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float pi = pp[i], mi = mm[i], vi = vv[i];
+      adam_value(pi, gg[i], mi, vi, c);
+      pp[i] = pi;
+      mm[i] = mi;
+      vv[i] = vi;
+    }
+    store4_part(p + e, pp, k);
+    store4_part(m + e, mm, k);
+    store4_part(v + e, vv, k);
+    if constexpr (!__is_same(LT, None)) store4_part(static_cast<LT*>(t.low) + base + e, pp, k);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// 8-bit moments.  A tensor of n values is ceil(n / 64) blocks; its form is 64 bytes of codes for each block and behind
+// them one float32 scale s for each, the largest magnitude of the block:
+//   first moment    m = +- s (k / 127)^2   code +-k, k = round(127 sqrt(|m| / s))
+//   second moment   v =    s (k / 255)^4   code   k, k = round(255 (v / s)^(1/4)), at least 1 for v > 0
+// Roots space the codes finer towards 0, evenly in relative terms over a range of 1.6e4 in m and 6e4 in sqrt(v); a
+// second moment over 0 never becomes 0, so no update divides by eps alone.  The rounding is to nearest: with stochastic
+// rounding the noise accumulates over 1 / (1 - beta2) steps and updates end up further from the 32-bit ones.
+// A block whose largest magnitude is below the smallest normal number is stored as 0, one that holds a value that is not
+// finite as NaN.  Codes of places behind the last value are 0.
+// ---------------------------------------------------------------------------------------------
+__host__ __device__ inline int64_t blocks8(int64_t n) { return (n + BLOCK8 - 1) / BLOCK8; }
+
+// Maximum over the 16 lanes of a row (a block is 16 lanes of 4 values): exchanges inside the row only, so every lane
+// of the row must be active.
+__device__ __forceinline__ uint32_t row_max(uint32_t x) {
+#define MI_ROW_STEP(ctrl) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, 0xf, 0xf, true))
+  MI_ROW_STEP(0xB1);   // quad_perm [1, 0, 3, 2]
+  MI_ROW_STEP(0x4E);   // quad_perm [2, 3, 0, 1]
+  MI_ROW_STEP(0x141);  // row_half_mirror: the other quad of eight lanes
+  MI_ROW_STEP(0x140);  // row_mirror: the other half of the row
+#undef MI_ROW_STEP
+  return x;
+}
+
+// Scale of the block this lane's four magnitudes belong to.  The bit patterns of magnitudes order as the numbers do,
+// with infinities and then NaN above every finite one.
+__device__ __forceinline__ float block_scale(f32x4_t x) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  top = row_max(top);
+  return top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : top < 0x00800000u ? 0.0f : __uint_as_float(top);
+}
+
+template <bool SIGNED>
+__device__ __forceinline__ uint32_t encode4(f32x4_t x, float s) {
+  uint32_t codes = 0;
+  const bool held = s > 0.0f;  // not for 0 and not for NaN
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float share = held ? fabsf(x[i]) / s : 0.0f;
+    if constexpr (SIGNED) {
+      int k = (int)rintf(sqrtf(share) * 127.0f);
+      if (x[i] < 0.0f) k = -k;
+      codes |= ((uint32_t)k & 0xffu) << (8 * i);
+    } else {
+      uint32_t k = (uint32_t)rintf(sqrtf(sqrtf(share)) * 255.0f);
+      if (held && x[i] > 0.0f) k = max(k, 1u);
+      codes |= (k & 0xffu) << (8 * i);
+    }
+  }
+  return codes;
+}
+template <bool SIGNED>
+__device__ __forceinline__ f32x4_t decode4(uint32_t codes, float s) {
+  f32x4_t x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    // the scale comes last: a share of it that is taken first would be denormal for scales far above the smallest number
+    if constexpr (SIGNED) {
+      const float k = (float)(int8_t)(codes >> (8 * i));
+      x[i] = k * fabsf(k) * (1.0f / (127 * 127)) * s;
+    } else {
+      const float k = (float)((codes >> (8 * i)) & 0xffu);
+      const float k2 = k * k * (1.0f / (255 * 255));
+      x[i] = k2 * k2 * s;
+    }
+  }
+  return x;
+}
+
+constexpr int ADAM8_U = 4;
+constexpr int ADAM8_CHUNK = NT * 4 * ADAM8_U;
+static_assert(ADAM8_CHUNK % BLOCK8 == 0, "chunks are whole blocks");
+
+template <class PT, class GT, class LT>
+__global__ __launch_bounds__(NT) void adamw8_kernel(AdamArgs a) {
+  const int ti = tensor_of(a.list, blockIdx.x);
+  const AdamTensor t = a.list.t[ti];
+  const int64_t base = (int64_t)(blockIdx.x - a.list.first[ti]) * ADAM8_CHUNK;
+  PT* __restrict__ p = static_cast<PT*>(t.p) + base;
+  const GT* __restrict__ g = static_cast<const GT*>(t.g) + base;
+  const int64_t nb = blocks8(t.n);
+  uint8_t* m8 = static_cast<uint8_t*>(t.m);
+  uint8_t* v8 = static_cast<uint8_t*>(t.v);
+  uint32_t* __restrict__ mc = reinterpret_cast<uint32_t*>(m8 + base);
+  uint32_t* __restrict__ vc = reinterpret_cast<uint32_t*>(v8 + base);
+  float* __restrict__ ms = reinterpret_cast<float*>(m8 + nb * BLOCK8) + base / BLOCK8;
+  float* __restrict__ vs = reinterpret_cast<float*>(v8 + nb * BLOCK8) + base / BLOCK8;
+  const int64_t left = t.n - base;
+  const AdamCoef c = adam_coefficients(a.s, t.step);
+  for (int u = 0; u < ADAM8_U; ++u) {
+    const int e = (u * NT + threadIdx.x) * 4;
+    const int b = e / BLOCK8;
+    if ((int64_t)b * BLOCK8 >= left) return;  // the whole row of 16 lanes, whose block this is
+    const int k = left - e >= 4 ? 4 : left - e > 0 ? (int)(left - e) : 0;
+    f32x4_t pp, gg;
+    if (k == 4) {
+      pp = load4(p + e);
+      gg = load4(g + e);
+    } else {
+      pp = load4_part(p + e, k);
+      gg = load4_part(g + e, k);
+    }
+    f32x4_t mm = decode4<true>(mc[e / 4], ms[b]), vv = decode4<false>(vc[e / 4], vs[b]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float pi = pp[i], mi = mm[i], vi = vv[i];
+      adam_value(pi, gg[i], mi, vi, c);
+      pp[i] = pi;
+      mm[i] = i < k ? mi : 0.0f;  // places behind the last value hold 0
+      vv[i] = i < k ? vi : 0.0f;
+    }
+    const float sm = block_scale(mm), sv = block_scale(vv);
+    mc[e / 4] = encode4<true>(mm, sm);
+    vc[e / 4] = encode4<false>(vv, sv);
+    if ((threadIdx.x & 15) == 0) {
+      ms[b] = sm;
+      vs[b] = sv;
+    }
+    if (k == 4) {
+      store4(p + e, pp);
+      if constexpr (!__is_same(LT, None)) store4(static_cast<LT*>(t.low) + base + e, pp);
+    } else {
+      store4_part(p + e, pp, k);
+      if constexpr (!__is_same(LT, None)) store4_part(static_cast<LT*>(t.low) + base + e, pp, k);
+    }
+  }
+}
+
+// Conversions between a list of tensors and their 8-bit forms.
+constexpr int MOVE_U = 4;
+constexpr int MOVE_CHUNK = NT * 4 * MOVE_U;
+
+template <class T, bool SIGNED>
+__global__ __launch_bounds__(NT) void pack8_kernel(MoveList l) {
+  const int ti = tensor_of(l, blockIdx.x);
+  const MoveTensor t = l.t[ti];
+  const int64_t base = (int64_t)(blockIdx.x - l.first[ti]) * MOVE_CHUNK;
+  const T* __restrict__ x = static_cast<const T*>(t.src) + base;
+  uint8_t* out = static_cast<uint8_t*>(t.dst);
+  uint32_t* __restrict__ codes = reinterpret_cast<uint32_t*>(out + base);
+  float* __restrict__ scales = reinterpret_cast<float*>(out + blocks8(t.n) * BLOCK8) + base / BLOCK8;
+  const int64_t left = t.n - base;
+  for (int u = 0; u < MOVE_U; ++u) {
+    const int e = (u * NT + threadIdx.x) * 4;
+    const int b = e / BLOCK8;
+    if ((int64_t)b * BLOCK8 >= left) return;  // the whole row of 16 lanes, whose block this is
+    const int k = left - e >= 4 ? 4 : left - e > 0 ? (int)(left - e) : 0;
+    const f32x4_t xx = k == 4 ? load4(x + e) : load4_part(x + e, k);
+    const float s = block_scale(xx);
+    codes[e / 4] = encode4<SIGNED>(xx, s);
+    if ((threadIdx.x & 15) == 0) scales[b] = s;
+  }
+}
+
+template <class T, bool SIGNED>
+__global__ __launch_bounds__(NT) void unpack8_kernel(MoveList l) {
+  const int ti = tensor_of(l, blockIdx.x);
+  const MoveTensor t = l.t[ti];
+  const int64_t base = (int64_t)(blockIdx.x - l.first[ti]) * MOVE_CHUNK;
+  const uint8_t* in = static_cast<const uint8_t*>(t.src);
+  const uint32_t* __restrict__ codes = reinterpret_cast<const uint32_t*>(in + base);
+  const float* __restrict__ scales = reinterpret_cast<const float*>(in + blocks8(t.n) * BLOCK8) + base / BLOCK8;
+  T* __restrict__ x = static_cast<T*>(t.dst) + base;
+  const int64_t left = t.n - base;
+  for (int u = 0; u < MOVE_U; ++u) {
+    const int e = (u * NT + threadIdx.x) * 4;
+    if (e >= left) return;
+    const f32x4_t xx = decode4<SIGNED>(codes[e / 4], scales[e / BLOCK8]);
+    if (left - e >= 4) store4(x + e, xx);
+    else store4_part(x + e, xx, (int)(left - e));
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Global norm and scaling
+// ---------------------------------------------------------------------------------------------
+constexpr int NORM_U = 16;
+constexpr int NORM_CHUNK = NT * 4 * NORM_U;
+
+__device__ __forceinline__ double wave_sum(double x) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d, 64);
+  return x;
+}
+// Sum over the workgroup, in thread 0, in a fixed order.
+template <int THREADS>
+__device__ __forceinline__ double group_sum(double x) {
+  __shared__ double part[THREADS / 64];
+  x = wave_sum(x);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+  __syncthreads();
+  double s = 0.0;
+  if (threadIdx.x == 0)
+    for (int w = 0; w < THREADS / 64; ++w) s += part[w];
+  return s;
+}
+
+// Sum of squares of every chunk, in 64 bits: squares of float32 values neither overflow nor vanish there, and sums over
+// a whole model lose nothing.
+template <class T>
+__global__ __launch_bounds__(NT) void sumsq_list_kernel(ReadList l, double* __restrict__ partials) {
+  const int ti = tensor_of(l, blockIdx.x);
+  const int64_t base = (int64_t)(blockIdx.x - l.first[ti]) * NORM_CHUNK;
+  const T* __restrict__ x = static_cast<const T*>(l.t[ti].x) + base;
+  const int64_t left = l.t[ti].n - base;
+  double sum = 0.0;
+  if (left >= NORM_CHUNK) {
+#pragma unroll 4
+    for (int u = 0; u < NORM_U; ++u) {
+      const f32x4_t xx = load4(x + (u * NT + threadIdx.x) * 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum = fma((double)xx[i], (double)xx[i], sum);
+    }
+  } else {
+    for (int64_t e = threadIdx.x * 4; e < left; e += NT * 4) {
+      const f32x4_t xx = load4_part(x + e, left - e < 4 ? (int)(left - e) : 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum = fma((double)xx[i], (double)xx[i], sum);
+    }
+  }
+  sum = group_sum<NT>(sum);
+  if (threadIdx.x == 0) partials[blockIdx.x] = sum;
+}
+
+// out[0] = norm, out[1] = min(1, max_norm / (norm + 1e-6)); a norm that is not a number makes the factor NaN.
+__global__ __launch_bounds__(1024) void norm_finish_kernel(const double* __restrict__ partials, int64_t count, float max_norm,
+                                                           float* __restrict__ out) {
+  double sum = 0.0;
+  for (int64_t i = threadIdx.x; i < count; i += 1024) sum += partials[i];
+  sum = group_sum<1024>(sum);
+  if (threadIdx.x == 0) {
+    const float norm = (float)sqrt(sum);
+    out[0] = norm;
+    const float f = max_norm / (norm + 1e-6f);
+    out[1] = f > 1.0f ? 1.0f : f;
+  }
+}
+
+constexpr int SCALE_U = 4;
+constexpr int SCALE_CHUNK = NT * 4 * SCALE_U;
+
+// x <- factor x; a factor of 1 changes nothing and reads nothing.
+template <class T>
+__global__ __launch_bounds__(NT) void scale_list_kernel(ReadList l, const float* __restrict__ factor) {
+  const float f = *factor;
+  if (f == 1.0f) return;
+  const int ti = tensor_of(l, blockIdx.x);
+  const int64_t base = (int64_t)(blockIdx.x - l.first[ti]) * SCALE_CHUNK;
+  T* __restrict__ x = static_cast<T*>(const_cast<void*>(l.t[ti].x)) + base;
+  const int64_t left = l.t[ti].n - base;
+  if (left >= SCALE_CHUNK) {
+    f32x4_t xx[SCALE_U];
+#pragma unroll
+    for (int u = 0; u < SCALE_U; ++u) xx[u] = load4(x + (u * NT + threadIdx.x) * 4);
+#pragma unroll
+    for (int u = 0; u < SCALE_U; ++u) store4(x + (u * NT + threadIdx.x) * 4, xx[u] * f);
+    return;
+  }
+  for (int64_t e = threadIdx.x * 4; e < left; e += NT * 4) {
+    const int k = left - e < 4 ? (int)(left - e) : 4;
+    store4_part(x + e, load4_part(x + e, k) * f, k);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------------
+// Walks a list of tensors and hands full argument blocks to `launch(list, chunks)`: empty tensors are left out, a block
+// ends when it is full or its chunks would be too many.  `fill(i)` makes the entry of tensor i.
+template <class L, class Fill, class Launch>
+int for_each_list(int64_t count, const int64_t* numel, int64_t chunk, L& list, Fill fill, Launch launch) {
+  int64_t chunks = 0;
+  list.count = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (numel[i] == 0) continue;
+    const int64_t c = (numel[i] + chunk - 1) / chunk;
+    if (list.count == L::CAPACITY || (list.count > 0 && chunks + c > MAX_CHUNKS)) {
+      if (int rc = launch(list, chunks)) return rc;
+      list.count = 0;
+      chunks = 0;
+    }
+    list.first[list.count] = (uint32_t)chunks;
+    list.t[list.count++] = fill(i);
+    chunks += c;
+  }
+  return list.count ? launch(list, chunks) : MI_OK;
+}
+
+int launched(const char* who) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? MI_OK : fail(MI_ERR_LAUNCH, "%s: launch failed: %s", who, hipGetErrorString(e));
+}
+
+#ifdef MI_HOST_CHECK
+// Every chunk of a launch falls into the tensor the bisection finds, at an offset inside it.
+template <class L>
+void walk(const L& l, int64_t chunks, int64_t chunk) {
+  for (int64_t b = 0; b < chunks; b += (chunks > 4096 && b > 64 && b < chunks - 64) ? 61 : 1) {
+    const int ti = tensor_of(l, (uint32_t)b);
+    if (ti < 0 || ti >= l.count || l.first[ti] > b) host_check::fail("a chunk without a tensor");
+    else if ((b - l.first[ti]) * chunk >= l.t[ti].n) host_check::fail("a chunk behind the end of its tensor");
+  }
+}
+#define MI_WALK(...) walk(__VA_ARGS__)
+#else
+#define MI_WALK(...) ((void)0)
+#endif
+
+int element_bytes(int dtype) { return dtype == MI_DTYPE_F32 ? 4 : 2; }
+bool known_dtype(int dtype) { return dtype == MI_DTYPE_F32 || dtype == MI_DTYPE_BF16 || dtype == MI_DTYPE_F16; }
+
+// Memory of a call: no written range may meet any other.
+struct Span {
+  uintptr_t lo, hi;
+  bool written;
+};
+bool spans_conflict(std::vector<Span>& spans) {
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
+  uintptr_t end_any = 0, end_written = 0;
+  for (const Span& s : spans) {
+    if (s.lo < (s.written ? end_any : end_written)) return true;
+    end_any = std::max(end_any, s.hi);
+    if (s.written) end_written = std::max(end_written, s.hi);
+  }
+  return false;
+}
+
+// Checks one list argument and adds its ranges.
+int add_spans(const char* who, const char* what, std::vector<Span>& spans, int64_t count, const void* const* ptrs, const int64_t* numel,
+              int bytes, bool packed, bool written) {
+  if (!ptrs && count > 0) return fail(MI_ERR_BAD_ARG, "%s: no list of %s", who, what);
+  const uintptr_t align = packed ? 16 : (uintptr_t)bytes;
+  for (int64_t i = 0; i < count; ++i) {
+    if (numel[i] == 0) continue;
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(ptrs[i]);
+    if (!lo) return fail(MI_ERR_BAD_ARG, "%s: %s %lld is null", who, what, (long long)i);
+    if (lo % align) return fail(MI_ERR_BAD_ARG, "%s: %s %lld is not aligned to %d bytes", who, what, (long long)i, (int)align);
+    spans.push_back({lo, lo + (packed ? mi_moment_8bit_bytes(numel[i]) : (size_t)numel[i] * bytes), written});
+  }
+  return MI_OK;
+}
+
+int check_numel(const char* who, int64_t count, const int64_t* numel) {
+  if (count < 0 || (count > 0 && !numel)) return fail(MI_ERR_BAD_ARG, "%s: bad tensor count or no sizes", who);
+  for (int64_t i = 0; i < count; ++i) {
+    if (numel[i] < 0) return fail(MI_ERR_BAD_ARG, "%s: tensor %lld has a negative size", who, (long long)i);
+    if (numel[i] > MAX_NUMEL)
+      return fail(MI_ERR_UNSUPPORTED_SHAPE, "%s: tensor %lld has %lld elements, at most 2^35 are supported", who, (long long)i, (long long)numel[i]);
+  }
+  return MI_OK;
+}
+
+template <class PT, class GT, class LT>
+int adam_launch(bool bits8, const AdamArgs& a, int64_t chunks, hipStream_t stream) {
+  const dim3 grid((unsigned)chunks), block(NT);
+  if (bits8) hipLaunchKernelGGL((adamw8_kernel<PT, GT, LT>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((adamw_kernel<PT, GT, LT>), grid, block, 0, stream, a);
+  return launched("mi_adamw_update");
+}
+template <class PT, class LT>
+int adam_launch_grad(int grad_dtype, bool bits8, const AdamArgs& a, int64_t chunks, hipStream_t stream) {
+  if (grad_dtype == MI_DTYPE_F32) return adam_launch<PT, float, LT>(bits8, a, chunks, stream);
+  if constexpr (!__is_same(PT, _Float16) && !__is_same(LT, _Float16))
+    if (grad_dtype == MI_DTYPE_BF16) return adam_launch<PT, __bf16, LT>(bits8, a, chunks, stream);
+  if constexpr (!__is_same(PT, __bf16) && !__is_same(LT, __bf16))
+    if (grad_dtype == MI_DTYPE_F16) return adam_launch<PT, _Float16, LT>(bits8, a, chunks, stream);
+  return fail(MI_ERR_BAD_ARG, "mi_adamw_update: bfloat16 and float16 do not go together");
+}
+
+int adam_impl(int64_t count, void* const* param, const void* const* grad, void* const* exp_avg, void* const* exp_avg_sq,
+              void* const* model_param, const float* const* step_dev, const int64_t* numel, int param_dtype, int grad_dtype, int model_dtype,
+              int moment_bits, double step, double lr, const float* lr_dev, double beta1, double beta2, double eps, double weight_decay,
+              int decay_method, const float* grad_scale, hipStream_t stream) {
+  const char* who = "mi_adamw_update";
+  if (int rc = check_numel(who, count, numel)) return rc;
+  if (!known_dtype(param_dtype) || !known_dtype(grad_dtype)) return fail(MI_ERR_BAD_ARG, "%s: unknown data type", who);
+  if (model_param && (param_dtype != MI_DTYPE_F32 || (model_dtype != MI_DTYPE_BF16 && model_dtype != MI_DTYPE_F16)))
+    return fail(MI_ERR_BAD_ARG, "%s: 16-bit copies go with float32 weights only", who);
+  const int mixed = model_param ? model_dtype : param_dtype;
+  if (mixed != MI_DTYPE_F32 && grad_dtype != MI_DTYPE_F32 && grad_dtype != mixed)
+    return fail(MI_ERR_BAD_ARG, "%s: bfloat16 and float16 do not go together", who);
+  if (moment_bits != 32 && moment_bits != 8) return fail(MI_ERR_BAD_ARG, "%s: moments have 32 or 8 bits, got %d", who, moment_bits);
+  // (comparisons that NaN fails)
+  if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0)) return fail(MI_ERR_BAD_ARG, "%s: betas must be in [0, 1)", who);
+  if (!(eps >= 0.0)) return fail(MI_ERR_BAD_ARG, "%s: eps must not be negative", who);
+  if (!step_dev && !(step >= 1.0)) return fail(MI_ERR_BAD_ARG, "%s: step must be at least 1", who);
+  if (decay_method < DECAY_DECOUPLED || decay_method > DECAY_PALM) return fail(MI_ERR_BAD_ARG, "%s: unknown weight decay method %d", who, decay_method);
+  const bool bits8 = moment_bits == 8;
+  const int pb = element_bytes(param_dtype), gb = element_bytes(grad_dtype);
+  {
+    std::vector<Span> spans;
+    spans.reserve((size_t)count * (model_param ? 5 : 4));
+    if (int rc = add_spans(who, "param", spans, count, const_cast<const void* const*>(param), numel, pb, false, true)) return rc;
+    if (int rc = add_spans(who, "grad", spans, count, grad, numel, gb, false, false)) return rc;
+    if (int rc = add_spans(who, "exp_avg", spans, count, const_cast<const void* const*>(exp_avg), numel, 4, bits8, true)) return rc;
+    if (int rc = add_spans(who, "exp_avg_sq", spans, count, const_cast<const void* const*>(exp_avg_sq), numel, 4, bits8, true)) return rc;
+    if (model_param)
+      if (int rc = add_spans(who, "model_param", spans, count, const_cast<const void* const*>(model_param), numel, 2, false, true)) return rc;
+    if (step_dev)
+      for (int64_t i = 0; i < count; ++i)
+        if (!step_dev[i] || reinterpret_cast<uintptr_t>(step_dev[i]) % 4) return fail(MI_ERR_BAD_ARG, "%s: step %lld is null or not aligned", who, (long long)i);
+    if (spans_conflict(spans)) return fail(MI_ERR_BAD_ARG, "%s: a tensor that is written overlaps another one of the call", who);
+  }
+  AdamArgs a = {};
+  AdamScalars& s = a.s;
+  s.b1 = (float)beta1;
+  s.omb1 = (float)(1.0 - beta1);
+  s.b2 = (float)beta2;
+  s.omb2 = (float)(1.0 - beta2);
+  s.eps = (float)eps;
+  s.on_device = step_dev || lr_dev;
+  s.method = decay_method;
+  s.lr = lr;
+  s.wd = weight_decay;
+  s.ln_b1 = log(beta1);
+  s.ln_b2 = log(beta2);
+  s.step = step;
+  s.lr_dev = lr_dev;
+  s.grad_scale = grad_scale;
+  decay_terms(decay_method, weight_decay, lr, &s.keep, &s.l2);
+  if (!step_dev) bias_terms(s.ln_b1, s.ln_b2, step, lr, &s.step_size, &s.inv_sqrt_bc2);
+  const int64_t chunk = bits8 ? ADAM8_CHUNK : ADAM_CHUNK;
+  return for_each_list(
+      count, numel, chunk, a.list,
+      [&](int64_t i) {
+        return AdamTensor{param[i], grad[i], exp_avg[i], exp_avg_sq[i], model_param ? model_param[i] : nullptr, step_dev ? step_dev[i] : nullptr, numel[i]};
+      },
+      [&](const AdamList& l, int64_t chunks) -> int {
+        MI_OTHER_LAUNCH();
+        MI_WALK(l, chunks, chunk);
+        for (int i = 0; i < l.count; ++i) {
+          [[maybe_unused]] const AdamTensor& t = l.t[i];
+          [[maybe_unused]] const int64_t bytes8 = (int64_t)mi_moment_8bit_bytes(t.n);
+          MI_FOOTPRINT("weights", t.p, pb, 1, t.n, 1, t.n, t.n);
+          MI_FOOTPRINT("gradient", t.g, gb, 1, t.n, 1, t.n, t.n);
+          MI_FOOTPRINT("first moment", t.m, bits8 ? 1 : 4, 1, 0, 1, bits8 ? bytes8 : t.n, bits8 ? bytes8 : t.n);
+          MI_FOOTPRINT("second moment", t.v, bits8 ? 1 : 4, 1, 0, 1, bits8 ? bytes8 : t.n, bits8 ? bytes8 : t.n);
+          MI_FOOTPRINT("16-bit copy", t.low, 2, 1, 0, 1, t.n, t.n);
+        }
+        if (model_param)
+          return model_dtype == MI_DTYPE_BF16 ? adam_launch_grad<float, __bf16>(grad_dtype, bits8, a, chunks, stream)
+                                              : adam_launch_grad<float, _Float16>(grad_dtype, bits8, a, chunks, stream);
+        if (param_dtype == MI_DTYPE_F32) return adam_launch_grad<float, None>(grad_dtype, bits8, a, chunks, stream);
+        if (param_dtype == MI_DTYPE_BF16) return adam_launch_grad<__bf16, None>(grad_dtype, bits8, a, chunks, stream);
+        return adam_launch_grad<_Float16, None>(grad_dtype, bits8, a, chunks, stream);
+      });
+}
+
+// Runs of equal data types are served by one launch each (as far as the argument block goes).
+template <class Body>
+int for_each_type(int64_t count, const int* dtype, Body body) {
+  for (int64_t i = 0; i < count;) {
+    int64_t j = i + 1;
+    while (j < count && dtype[j] == dtype[i]) ++j;
+    if (int rc = body(i, j - i, dtype[i])) return rc;
+    i = j;
+  }
+  return MI_OK;
+}
+
+int64_t norm_chunks(int64_t count, const int64_t* numel) {
+  int64_t chunks = 0;
+  for (int64_t i = 0; i < count; ++i) chunks += (numel[i] + NORM_CHUNK - 1) / NORM_CHUNK;
+  return chunks;
+}
+
+int check_list(const char* who, int64_t count, const void* const* x, const int64_t* numel, const int* dtype) {
+  if (int rc = check_numel(who, count, numel)) return rc;
+  if (count > 0 && (!x || !dtype)) return fail(MI_ERR_BAD_ARG, "%s: no list of tensors or data types", who);
+  for (int64_t i = 0; i < count; ++i) {
+    if (!known_dtype(dtype[i])) return fail(MI_ERR_BAD_ARG, "%s: tensor %lld has an unknown data type", who, (long long)i);
+    if (numel[i] > 0 && (!x[i] || reinterpret_cast<uintptr_t>(x[i]) % element_bytes(dtype[i])))
+      return fail(MI_ERR_BAD_ARG, "%s: tensor %lld is null or not aligned to its elements", who, (long long)i);
+  }
+  return MI_OK;
+}
+
+int norm_impl(int64_t count, const void* const* x, const int64_t* numel, const int* dtype, double max_norm, double* partials, size_t partials_len,
+              float* out, hipStream_t stream) {
+  const char* who = "mi_global_norm";
+  if (int rc = check_list(who, count, x, numel, dtype)) return rc;
+  if (!out) return fail(MI_ERR_BAD_ARG, "%s: no output", who);
+  if (!(max_norm >= 0.0)) return fail(MI_ERR_BAD_ARG, "%s: max_norm must not be negative", who);
+  const int64_t total = norm_chunks(count, numel);
+  if (total > 0 && (!partials || partials_len < (size_t)total))
+    return fail(MI_ERR_WORKSPACE, "%s: %lld partial sums are needed", who, (long long)total);
+  MI_FOOTPRINT("partial sums", partials, 8, 1, 0, 1, total, total);
+  MI_FOOTPRINT("norm and factor", out, 4, 1, 0, 1, 2, 2);
+  int64_t done = 0;
+  ReadList l;
+  const int rc = for_each_type(count, dtype, [&](int64_t at, int64_t len, int dt) {
+    return for_each_list(
+        len, numel + at, NORM_CHUNK, l, [&](int64_t i) { return ReadTensor{x[at + i], numel[at + i]}; },
+        [&](const ReadList& list, int64_t chunks) -> int {
+          MI_OTHER_LAUNCH();
+          MI_WALK(list, chunks, NORM_CHUNK);
+          for (int i = 0; i < list.count; ++i) MI_FOOTPRINT("tensor", list.t[i].x, element_bytes(dt), 1, 0, 1, list.t[i].n, list.t[i].n);
+          const dim3 grid((unsigned)chunks), block(NT);
+          if (dt == MI_DTYPE_F32) hipLaunchKernelGGL(sumsq_list_kernel<float>, grid, block, 0, stream, list, partials + done);
+          else if (dt == MI_DTYPE_BF16) hipLaunchKernelGGL(sumsq_list_kernel<__bf16>, grid, block, 0, stream, list, partials + done);
+          else hipLaunchKernelGGL(sumsq_list_kernel<_Float16>, grid, block, 0, stream, list, partials + done);
+          done += chunks;
+          return launched(who);
+        });
+  });
+  if (rc != MI_OK) return rc;
+  MI_OTHER_LAUNCH();
+  hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(1024), 0, stream, partials, total, (float)max_norm, out);
+  return launched(who);
+}
+
+int scale_impl(int64_t count, void* const* x, const int64_t* numel, const int* dtype, const float* factor, hipStream_t stream) {
+  const char* who = "mi_scale_tensors";
+  if (int rc = check_list(who, count, const_cast<const void* const*>(x), numel, dtype)) return rc;
+  if (!factor) return fail(MI_ERR_BAD_ARG, "%s: no factor", who);
+  std::vector<Span> spans;
+  spans.reserve((size_t)count);
+  for (int64_t i = 0; i < count; ++i) {
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(x[i]);
+    if (numel[i] > 0) spans.push_back({lo, lo + (size_t)numel[i] * element_bytes(dtype[i]), true});
+  }
+  if (spans_conflict(spans)) return fail(MI_ERR_BAD_ARG, "%s: two of the tensors overlap", who);
+  ReadList l;
+  return for_each_type(count, dtype, [&](int64_t at, int64_t len, int dt) {
+    return for_each_list(
+        len, numel + at, SCALE_CHUNK, l, [&](int64_t i) { return ReadTensor{x[at + i], numel[at + i]}; },
+        [&](const ReadList& list, int64_t chunks) -> int {
+          MI_OTHER_LAUNCH();
+          MI_WALK(list, chunks, SCALE_CHUNK);
+          for (int i = 0; i < list.count; ++i) MI_FOOTPRINT("tensor", list.t[i].x, element_bytes(dt), 1, 0, 1, list.t[i].n, list.t[i].n);
+          const dim3 grid((unsigned)chunks), block(NT);
+          if (dt == MI_DTYPE_F32) hipLaunchKernelGGL(scale_list_kernel<float>, grid, block, 0, stream, list, factor);
+          else if (dt == MI_DTYPE_BF16) hipLaunchKernelGGL(scale_list_kernel<__bf16>, grid, block, 0, stream, list, factor);
+          else hipLaunchKernelGGL(scale_list_kernel<_Float16>, grid, block, 0, stream, list, factor);
+          return launched(who);
+        });
+  });
+}
+
+template <class T>
+int move_launch(bool pack, bool second, const MoveList& l, int64_t chunks, hipStream_t stream, const char* who) {
+  const dim3 grid((unsigned)chunks), block(NT);
+  if (pack && !second) hipLaunchKernelGGL((pack8_kernel<T, true>), grid, block, 0, stream, l);
+  else if (pack) hipLaunchKernelGGL((pack8_kernel<T, false>), grid, block, 0, stream, l);
+  else if (!second) hipLaunchKernelGGL((unpack8_kernel<T, true>), grid, block, 0, stream, l);
+  else hipLaunchKernelGGL((unpack8_kernel<T, false>), grid, block, 0, stream, l);
+  return launched(who);
+}
+
+int move_impl(bool pack, int64_t count, const void* const* src, void* const* dst, const int64_t* numel, int dtype, int second, hipStream_t stream) {
+  const char* who = pack ? "mi_moments_8bit_pack" : "mi_moments_8bit_unpack";
+  if (int rc = check_numel(who, count, numel)) return rc;
+  if (!known_dtype(dtype)) return fail(MI_ERR_BAD_ARG, "%s: unknown data type", who);
+  if (second != 0 && second != 1) return fail(MI_ERR_BAD_ARG, "%s: the moment is 0 (first) or 1 (second), got %d", who, second);
+  {
+    std::vector<Span> spans;
+    spans.reserve((size_t)count * 2);
+    if (int rc = add_spans(who, "source", spans, count, src, numel, element_bytes(dtype), !pack, false)) return rc;
+    if (int rc = add_spans(who, "destination", spans, count, const_cast<const void* const*>(dst), numel, element_bytes(dtype), pack, true)) return rc;
+    if (spans_conflict(spans)) return fail(MI_ERR_BAD_ARG, "%s: a tensor that is written overlaps another one of the call", who);
+  }
+  MoveList l;
+  return for_each_list(
+      count, numel, MOVE_CHUNK, l, [&](int64_t i) { return MoveTensor{src[i], dst[i], numel[i]}; },
+      [&](const MoveList& list, int64_t chunks) -> int {
+        MI_OTHER_LAUNCH();
+        MI_WALK(list, chunks, MOVE_CHUNK);
+        for (int i = 0; i < list.count; ++i) {
+          [[maybe_unused]] const MoveTensor& t = list.t[i];
+          [[maybe_unused]] const int64_t bytes8 = (int64_t)mi_moment_8bit_bytes(t.n);
+          MI_FOOTPRINT("8-bit form", pack ? t.dst : t.src, 1, 1, 0, 1, bytes8, bytes8);
+          MI_FOOTPRINT("values", pack ? t.src : t.dst, element_bytes(dtype), 1, 0, 1, t.n, t.n);
+        }
+        if (dtype == MI_DTYPE_F32) return move_launch<float>(pack, second != 0, list, chunks, stream, who);
+        if (dtype == MI_DTYPE_BF16) return move_launch<__bf16>(pack, second != 0, list, chunks, stream, who);
+        return move_launch<_Float16>(pack, second != 0, list, chunks, stream, who);
+      });
+}
+
+// The checks above keep vectors; nothing may be thrown across the C boundary.
+template <class Body>
+int guarded(const char* who, Body body) {
+  try {
+    return body();
+  } catch (const std::bad_alloc&) {
+    return fail(MI_ERR_BAD_ARG, "%s: out of host memory", who);
+  }
+}
+
+}  // namespace
+}  // namespace mi
+
+#pragma GCC visibility push(default)
+extern "C" {
+
+size_t mi_moment_8bit_bytes(int64_t numel) { return numel <= 0 ? 0 : (size_t)mi::blocks8(numel) * (mi::BLOCK8 + 4); }
+
+int mi_adamw_update(int64_t count, void* const* param, const void* const* grad, void* const* exp_avg, void* const* exp_avg_sq,
+                    void* const* model_param, const float* const* step_dev, const int64_t* numel, int param_dtype, int grad_dtype,
+                    int model_dtype, int moment_bits, double step, double lr, const float* lr_dev, double beta1, double beta2, double eps,
+                    double weight_decay, int decay_method, const float* grad_scale, void* stream) {
+  return mi::guarded("mi_adamw_update", [&] {
+    return mi::adam_impl(count, param, grad, exp_avg, exp_avg_sq, model_param, step_dev, numel, param_dtype, grad_dtype, model_dtype, moment_bits, step,
+                         lr, lr_dev, beta1, beta2, eps, weight_decay, decay_method, grad_scale, static_cast<hipStream_t>(stream));
+  });
+}
+
+size_t mi_global_norm_partials_len(int64_t count, const int64_t* numel) {
+  return count <= 0 || !numel ? 0 : (size_t)mi::norm_chunks(count, numel);
+}
+
+int mi_global_norm(int64_t count, const void* const* x, const int64_t* numel, const int* dtype, double max_norm, double* partials,
+                   size_t partials_len, float* out, void* stream) {
+  return mi::norm_impl(count, x, numel, dtype, max_norm, partials, partials_len, out, static_cast<hipStream_t>(stream));
+}
+
+int mi_scale_tensors(int64_t count, void* const* x, const int64_t* numel, const int* dtype, const float* factor, void* stream) {
+  return mi::guarded("mi_scale_tensors", [&] { return mi::scale_impl(count, x, numel, dtype, factor, static_cast<hipStream_t>(stream)); });
+}
+
+int mi_moments_8bit_pack(int64_t count, const void* const* src, void* const* packed, const int64_t* numel, int dtype, int second_moment, void* stream) {
+  return mi::guarded("mi_moments_8bit_pack",
+                     [&] { return mi::move_impl(true, count, src, packed, numel, dtype, second_moment, static_cast<hipStream_t>(stream)); });
+}
+
+int mi_moments_8bit_unpack(int64_t count, const void* const* packed, void* const* dst, const int64_t* numel, int dtype, int second_moment, void* stream) {
+  return mi::guarded("mi_moments_8bit_unpack",
+                     [&] { return mi::move_impl(false, count, packed, dst, numel, dtype, second_moment, static_cast<hipStream_t>(stream)); });
+}
+
+}  // extern "C"
+#pragma GCC visibility pop

@@ -28,6 +28,7 @@ MI_ERR_WORKSPACE = -4
 
 # Every symbol include/mi_ns.h declares: (name, restype, argtypes)
 _i64, _int, _f32, _vp, _sz = ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
+_f64 = ctypes.c_double
 EXPORTS = (
     ("mi_version", _int, ()),
     ("mi_last_error", ctypes.c_char_p, ()),
@@ -54,6 +55,17 @@ EXPORTS = (
         _int,
         (_vp, _vp, _vp, _i64, _i64, _i64, _f32, _int, _f32, _f32, _vp, _int, _f32, _int, _vp, _sz, _vp),
     ),
+    (
+        "mi_adamw_update",
+        _int,
+        (_i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _int, _f64, _f64, _vp, _f64, _f64, _f64, _f64, _int, _vp, _vp),
+    ),
+    ("mi_global_norm_partials_len", _sz, (_i64, _vp)),
+    ("mi_global_norm", _int, (_i64, _vp, _vp, _vp, _f64, _vp, _sz, _vp, _vp)),
+    ("mi_scale_tensors", _int, (_i64, _vp, _vp, _vp, _vp, _vp)),
+    ("mi_moment_8bit_bytes", _sz, (_i64,)),
+    ("mi_moments_8bit_pack", _int, (_i64, _vp, _vp, _vp, _int, _int, _vp)),
+    ("mi_moments_8bit_unpack", _int, (_i64, _vp, _vp, _vp, _int, _int, _vp)),
     ("mi_profile_begin", _int, ()),
     ("mi_profile_end", _int, (_vp, _vp)),
     ("mi_debug_last_launch", _int, (_vp, _vp, _vp, _vp)),

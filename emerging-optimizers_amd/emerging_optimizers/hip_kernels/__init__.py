@@ -1,7 +1,16 @@
-"""Python entry points of the gfx950 kernels (SYRK, GEMM+AXPY, Frobenius normalise, fused Newton-Schulz)."""
+"""Python entry points of the gfx950 kernels (SYRK, GEMM+AXPY, Frobenius normalise, fused Newton-Schulz, AdamW over
+lists of tensors)."""
 
 from .. import _hip
+from .adamw import (
+    fused_adamw_update,
+    fused_adamw_update_8bit,
+    moment_8bit_bytes,
+    pack_moments_8bit,
+    unpack_moments_8bit,
+)
 from .batched_syrk import batched_tsyrk_ex, can_use_batched_tsyrk
+from .grad_norm import clip_grads_by_global_norm, global_grad_norm, scale_tensors
 from .newton_schulz import (
     frob_normalize,
     fused_muon_update,
@@ -24,13 +33,21 @@ __all__ = [
     "HAS_TRITON_340",
     "batched_tsyrk_ex",
     "can_use_batched_tsyrk",
+    "clip_grads_by_global_norm",
     "frob_normalize",
+    "fused_adamw_update",
+    "fused_adamw_update_8bit",
     "fused_muon_update",
     "fused_newton_schulz",
     "fused_supported",
     "gemm_axpy",
+    "global_grad_norm",
+    "moment_8bit_bytes",
     "on_kernel_device",
+    "pack_moments_8bit",
     "require_library",
+    "scale_tensors",
     "tsyrk_ex",
     "tsyrk_ex_small_matrix",
+    "unpack_moments_8bit",
 ]

@@ -1,0 +1,210 @@
+"""AdamW over lists of tensors: moments in 32 or in 8 bits, and the conversions of 8-bit moments."""
+
+from __future__ import annotations
+
+from typing import Literal, Optional, Sequence, Union
+
+import torch
+
+from .. import _hip
+from . import _launch
+
+
+__all__ = ["fused_adamw_update", "fused_adamw_update_8bit", "moment_8bit_bytes", "pack_moments_8bit", "unpack_moments_8bit"]
+
+MomentT = Literal["exp_avg", "exp_avg_sq"]
+
+_DECAY_METHODS = {"decoupled": 0, "independent": 1, "l2": 2, "palm": 3}
+_MOMENTS = {"exp_avg": 0, "exp_avg_sq": 1}
+
+
+def moment_8bit_bytes(numel: int) -> int:
+    """Bytes of the 8-bit form of a moment of ``numel`` values: 64 codes and a float32 scale for each block of 64."""
+    return -(-numel // 64) * 68
+
+
+def _check_packed(who: str, what: str, packed: Sequence[torch.Tensor], like: Sequence[torch.Tensor]) -> None:
+    if len(packed) != len(like):
+        raise ValueError(f"{who}: {len(packed)} {what} for {len(like)} tensors")
+    for i, (t, p) in enumerate(zip(packed, like)):
+        if t.dtype != torch.uint8:
+            raise TypeError(f"{who}: {what}[{i}] must be uint8, got {t.dtype}")
+        if t.numel() != moment_8bit_bytes(p.numel()) or not t.is_contiguous():
+            raise ValueError(f"{who}: {what}[{i}] must be {moment_8bit_bytes(p.numel())} contiguous bytes, got {tuple(t.shape)}")
+
+
+def _device_scalar(who: str, what: str, t: torch.Tensor, device: int) -> torch.Tensor:
+    if t.dtype != torch.float32 or t.numel() != 1 or t.get_device() != device:
+        raise ValueError(f"{who}: {what} must be one float32 value on the GPU of the params, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t
+
+
+def _adamw(
+    who: str,
+    bits: int,
+    params: Sequence[torch.Tensor],
+    grads: Sequence[torch.Tensor],
+    exp_avgs: Sequence[torch.Tensor],
+    exp_avg_sqs: Sequence[torch.Tensor],
+    step: Union[float, Sequence[torch.Tensor]],
+    lr: Union[float, torch.Tensor],
+    beta1: float,
+    beta2: float,
+    eps: float,
+    weight_decay: float,
+    weight_decay_method: str,
+    grad_scale: Optional[torch.Tensor],
+    model_params: Optional[Sequence[torch.Tensor]],
+) -> None:
+    method = _DECAY_METHODS.get(weight_decay_method)
+    if method is None:
+        raise ValueError(f"Invalid weight decay method: {weight_decay_method}")
+    if len(params) == 0 and len(grads) == len(exp_avgs) == len(exp_avg_sqs) == len(model_params or ()) == 0:
+        return
+    p_type = _launch.list_dtype(who, "params", params)
+    g_type = _launch.list_dtype(who, "grads", grads)
+    _launch.check_like(who, "grads", grads, params)
+    if bits == 32:
+        for what, moments in (("exp_avgs", exp_avgs), ("exp_avg_sqs", exp_avg_sqs)):
+            _launch.list_dtype(who, what, moments, (torch.float32,))
+            _launch.check_like(who, what, moments, params)
+    else:
+        _check_packed(who, "exp_avgs", exp_avgs, params)
+        _check_packed(who, "exp_avg_sqs", exp_avg_sqs, params)
+    low_type = torch.bfloat16
+    if model_params is not None:
+        if p_type != torch.float32:
+            raise TypeError(f"{who}: model_params go with float32 params, got {p_type}")
+        low_type = _launch.list_dtype(who, "model_params", model_params, (torch.bfloat16, torch.float16))
+        _launch.check_like(who, "model_params", model_params, params)
+    device = _launch.list_device(who, params, grads, exp_avgs, exp_avg_sqs, model_params or ())
+    steps = None
+    if not isinstance(step, (int, float)):
+        if len(step) != len(params):
+            raise ValueError(f"{who}: {len(step)} steps for {len(params)} params")
+        steps = _launch.pointers([_device_scalar(who, "step", t, device) for t in step])
+    lr_ptr = None
+    if isinstance(lr, torch.Tensor):
+        lr_ptr, lr = _device_scalar(who, "lr", lr, device).data_ptr(), 0.0
+    scale_ptr = None if grad_scale is None else _device_scalar(who, "grad_scale", grad_scale, device).data_ptr()
+    lists = [_launch.pointers(t) for t in (params, grads, exp_avgs, exp_avg_sqs)]
+    low = None if model_params is None else _launch.pointers(model_params)
+    numels = _launch.array.array("q", map(torch.Tensor.numel, params))
+    with _launch.on_device(device):
+        rc = _hip.lib().mi_adamw_update(
+            len(params), *map(_launch.address, lists), _launch.address(low), _launch.address(steps), _launch.address(numels),
+            _launch.DTYPE_CODES[p_type], _launch.DTYPE_CODES[g_type], _launch.DTYPE_CODES[low_type], bits,
+            1.0 if steps is not None else float(step), float(lr), lr_ptr, float(beta1), float(beta2), float(eps),
+            float(weight_decay), method, scale_ptr, torch.cuda.current_stream().cuda_stream,
+        )  # fmt: skip
+    _hip.check(rc)
+
+
+def fused_adamw_update(
+    params: Sequence[torch.Tensor],
+    grads: Sequence[torch.Tensor],
+    exp_avgs: Sequence[torch.Tensor],
+    exp_avg_sqs: Sequence[torch.Tensor],
+    *,
+    step: Union[float, Sequence[torch.Tensor]],
+    lr: Union[float, torch.Tensor],
+    beta1: float,
+    beta2: float,
+    eps: float = 1e-8,
+    weight_decay: float = 0.0,
+    weight_decay_method: str = "decoupled",
+    grad_scale: Optional[torch.Tensor] = None,
+    model_params: Optional[Sequence[torch.Tensor]] = None,
+) -> None:
+    """One AdamW step of every tensor of ``params``, in place, with float32 moments (see ``mi_adamw_update``).
+
+    ``g = grad_scale * grad`` (plus ``weight_decay * p`` for the method "l2"); ``m = beta1 * m + (1 - beta1) * g``;
+    ``v = beta2 * v + (1 - beta2) * g**2``; ``p = keep * p - lr / (1 - beta1**t) * m / (sqrt(v / (1 - beta2**t)) + eps)``
+    with ``keep`` by weight-decay method as in :class:`~emerging_optimizers.mixin.WeightDecayMixin`.  Everything is
+    computed in float32 and rounded once.
+
+    Args:
+        params: weights of record; float32, bfloat16 or float16, one type a call, on one GPU
+        grads: gradients; float32 or, where weights or ``model_params`` have 16 bits, that type; with float32 weights
+            alone any of the three
+        exp_avgs: first moments, float32
+        exp_avg_sqs: second moments, float32
+        step: number of this step, from 1; or one float32 tensor on the GPU for each param (captured graphs)
+        lr: learning rate, a number or one float32 value on the GPU
+        weight_decay_method: "decoupled", "independent", "l2" or "palm"
+        grad_scale: one float32 value on the GPU that multiplies the gradients (``grads`` themselves stay as they are)
+        model_params: 16-bit copies of float32 ``params``, written only
+
+    Gradients, moments and copies have the shape of their param and fill their memory in its order; no tensor that is
+    written may share memory with another one.  Any size from 0 on, any alignment.  The work is enqueued on the current
+    stream of the tensors' GPU; nothing waits.
+    """
+    _adamw(
+        "fused_adamw_update", 32, params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps, weight_decay,
+        weight_decay_method, grad_scale, model_params,
+    )  # fmt: skip
+
+
+def fused_adamw_update_8bit(
+    params: Sequence[torch.Tensor],
+    grads: Sequence[torch.Tensor],
+    exp_avgs: Sequence[torch.Tensor],
+    exp_avg_sqs: Sequence[torch.Tensor],
+    *,
+    step: Union[float, Sequence[torch.Tensor]],
+    lr: Union[float, torch.Tensor],
+    beta1: float,
+    beta2: float,
+    eps: float = 1e-8,
+    weight_decay: float = 0.0,
+    weight_decay_method: str = "decoupled",
+    grad_scale: Optional[torch.Tensor] = None,
+    model_params: Optional[Sequence[torch.Tensor]] = None,
+) -> None:
+    """:func:`fused_adamw_update` with moments in their 8-bit form: ``exp_avgs`` and ``exp_avg_sqs`` are uint8 tensors
+    of :func:`moment_8bit_bytes` bytes each, 16-byte aligned (zeros stand for zero moments; see
+    :func:`pack_moments_8bit`).  The update uses the new moments before they are rounded to 8 bits.
+    """
+    _adamw(
+        "fused_adamw_update_8bit", 8, params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps, weight_decay,
+        weight_decay_method, grad_scale, model_params,
+    )  # fmt: skip
+
+
+def _move(who: str, pack: bool, values: Sequence[torch.Tensor], packed: Sequence[torch.Tensor], which: MomentT) -> None:
+    second = _MOMENTS.get(which)
+    if second is None:
+        raise ValueError(f'{who}: which must be "exp_avg" or "exp_avg_sq", got {which!r}')
+    _check_packed(who, "packed", packed, values)
+    if len(values) == 0:
+        return
+    dtype = _launch.list_dtype(who, "moments", values)
+    if not all(map(_launch.is_dense, values)):
+        raise ValueError(f"{who}: moments must fill their memory")
+    device = _launch.list_device(who, values, packed)
+    v, q = _launch.pointers(values), _launch.pointers(packed)
+    numels = _launch.array.array("q", map(torch.Tensor.numel, values))
+    src, dst = (v, q) if pack else (q, v)
+    lib = _hip.lib()
+    with _launch.on_device(device):
+        rc = (lib.mi_moments_8bit_pack if pack else lib.mi_moments_8bit_unpack)(
+            len(values), _launch.address(src), _launch.address(dst), _launch.address(numels), _launch.DTYPE_CODES[dtype], second,
+            torch.cuda.current_stream().cuda_stream,
+        )  # fmt: skip
+    _hip.check(rc)
+
+
+def pack_moments_8bit(moments: Sequence[torch.Tensor], packed: Sequence[torch.Tensor], *, which: MomentT) -> None:
+    """Writes the 8-bit form of every tensor of ``moments`` (float32, bfloat16 or float16) to its uint8 tensor of
+    :func:`moment_8bit_bytes` bytes in ``packed``.
+
+    The values, in memory order, are cut into blocks of 64 whose largest magnitude ``s`` is kept in float32.  ``which``
+    is "exp_avg" (codes ``k`` from -127 to 127 for ``sign(k) * s * (k / 127)**2``) or "exp_avg_sq" (codes from 0 to 255
+    for ``s * (k / 255)**4``, never 0 for a value over 0).  A block that holds a value that is not finite becomes NaN.
+    """
+    _move("pack_moments_8bit", True, moments, packed, which)
+
+
+def unpack_moments_8bit(packed: Sequence[torch.Tensor], moments: Sequence[torch.Tensor], *, which: MomentT) -> None:
+    """Writes the values that the 8-bit forms ``packed`` stand for to ``moments`` (float32, bfloat16 or float16)."""
+    _move("unpack_moments_8bit", False, moments, packed, which)

@@ -1,0 +1,268 @@
+"""AdamW for the parameters that are not orthogonalised: embeddings, the output head, gains and biases.
+
+All parameters of one kind are updated by one multi-tensor call (``hip_kernels.fused_adamw_update`` or, with
+``moment_bits=8``, ``hip_kernels.fused_adamw_update_8bit``).  The reference leaves these parameters to
+``torch.optim.AdamW``; the defaults and the names of the state's entries are those of that class, so checkpoints move
+in both directions.  Weight decay has the methods of the other optimizers of this package.
+
+On the CPU, on GPUs other than gfx950 and for float64 parameters the same formulas run as torch statements.
+"""
+
+from __future__ import annotations
+
+from typing import Any, Callable, Optional
+
+import torch
+from torch.optim.optimizer import Optimizer, ParamsT
+
+from emerging_optimizers import hip_kernels
+from emerging_optimizers.hip_kernels._launch import DTYPE_CODES, is_dense
+from emerging_optimizers.mixin import WeightDecayMixin, WeightDecayT
+
+
+__all__ = ["AdamW"]
+
+_BLOCK = 64  # values that share a scale in the 8-bit form of a moment
+_SMALLEST = torch.finfo(torch.float32).tiny
+
+
+def _pack_torch(x: torch.Tensor, which: str) -> torch.Tensor:
+    """``hip_kernels.pack_moments_8bit`` as torch statements: the 8-bit form of the flat float32 ``x``."""
+    blocks = torch.nn.functional.pad(x, (0, -x.numel() % _BLOCK)).view(-1, _BLOCK)
+    scale = blocks.abs().amax(1, keepdim=True)
+    scale = torch.where(scale.isfinite(), torch.where(scale < _SMALLEST, 0.0, scale), torch.nan)
+    share = torch.where(scale > 0, blocks.abs() / scale, 0.0)
+    if which == "exp_avg":
+        codes = ((share.sqrt() * 127).round() * blocks.sign()).nan_to_num().to(torch.int8).view(torch.uint8)
+    else:
+        codes = (share.sqrt().sqrt() * 255).round()
+        codes = torch.where((scale > 0) & (blocks > 0), codes.clamp_min(1), codes).nan_to_num().to(torch.uint8)
+    return torch.cat([codes.view(-1), scale.view(-1).view(torch.uint8)])
+
+
+def _unpack_torch(packed: torch.Tensor, numel: int, which: str) -> torch.Tensor:
+    """``hip_kernels.unpack_moments_8bit`` as torch statements: flat float32 values."""
+    size = packed.numel() // (_BLOCK + 4) * _BLOCK
+    codes, scale = packed[:size], packed[size:].clone().view(torch.float32).repeat_interleave(_BLOCK)
+    if which == "exp_avg":
+        k = codes.view(torch.int8).float()
+        return (k * k.abs() * (1 / 127**2) * scale)[:numel]
+    k = codes.float().square() * (1 / 255**2)
+    return (k * k * scale)[:numel]
+
+
+def _memory_order(t: torch.Tensor) -> torch.Tensor:
+    """Flat view of a dense tensor in the order of its memory."""
+    return t.as_strided((t.numel(),), (1,))
+
+
+class AdamW(WeightDecayMixin, Optimizer):
+    """Adam with decoupled weight decay (arXiv:1711.05101), one call for all parameters of a kind.
+
+    Args:
+        params: parameters (or parameter-group dicts) to optimize; float32, bfloat16 or float16 on a gfx950 GPU run on
+            the kernels
+        lr: learning rate; a number or, with ``capturable``, also one float32 value on the GPU
+        betas: EMA coefficients of gradient and squared gradient
+        eps: added to the square root of the second moment
+        weight_decay: weight-decay strength; how it is applied is set by ``weight_decay_method``
+        weight_decay_method: one of the flavours of :class:`~emerging_optimizers.mixin.WeightDecayMixin`
+        moment_bits: 32 for float32 moments, 8 for one byte a value and a float32 scale for each 64 values
+            (``hip_kernels.pack_moments_8bit``); 8 saves 5.9 bytes a parameter, and updates differ from the 32-bit
+            ones by a few per cent
+        master_weights: keep float32 weights of record for 16-bit parameters (in the state, as ``master``)
+        capturable: keep the step count on the GPU, so that a captured ``step()`` counts on when it is replayed
+    """
+
+    def __init__(
+        self,
+        params: ParamsT,
+        lr: float = 1e-3,
+        betas: tuple[float, float] = (0.9, 0.999),
+        eps: float = 1e-8,
+        weight_decay: float = 0.01,
+        *,
+        weight_decay_method: WeightDecayT = "decoupled",
+        moment_bits: int = 32,
+        master_weights: bool = False,
+        capturable: bool = False,
+    ) -> None:
+        if not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0:
+            raise ValueError(f"betas must be in [0, 1), got {betas}")
+        if not eps >= 0.0:
+            raise ValueError(f"eps must not be negative, got {eps}")
+        if moment_bits not in (8, 32):
+            raise ValueError(f"moment_bits must be 8 or 32, got {moment_bits}")
+        if isinstance(lr, torch.Tensor) and not capturable:
+            raise ValueError("a learning rate in a tensor needs capturable=True")
+        if weight_decay_method not in ("decoupled", "independent", "l2", "palm"):
+            raise ValueError(f"Invalid weight decay method: {weight_decay_method}")
+        self.weight_decay_method = weight_decay_method
+        self.moment_bits = moment_bits
+        self.master_weights = bool(master_weights)
+        self.capturable = bool(capturable)
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+
+    def _moment(self, p: torch.Tensor) -> torch.Tensor:
+        """A zero moment of ``p``."""
+        if self.moment_bits == 8:
+            return torch.zeros(hip_kernels.moment_8bit_bytes(p.numel()), dtype=torch.uint8, device=p.device)
+        return torch.zeros_like(p, dtype=torch.promote_types(p.dtype, torch.float32))
+
+    def _first_step(self, p: torch.Tensor) -> Any:
+        return torch.zeros((), dtype=torch.float32, device=p.device) if self.capturable else 0
+
+    @torch.no_grad()
+    def _init_group(self, group: dict, skip_non_grad_params: bool = True) -> None:
+        """Creates the state of every parameter of ``group`` that does not have one yet."""
+        for p in group["params"]:
+            if p.grad is None and skip_non_grad_params:
+                continue
+            state = self.state[p]
+            if state:
+                continue
+            if not is_dense(p):
+                raise ValueError("AdamW needs parameters that fill their memory")
+            if self.moment_bits == 8 and p.dtype not in DTYPE_CODES:
+                raise ValueError(f"8-bit moments need float32, bfloat16 or float16 parameters, got {p.dtype}")
+            state["step"] = self._first_step(p)
+            state["exp_avg"] = self._moment(p)
+            state["exp_avg_sq"] = self._moment(p)
+            if self.master_weights and p.dtype in (torch.bfloat16, torch.float16):
+                state["master"] = p.detach().to(torch.float32)
+
+    @torch.no_grad()
+    def step(self, closure: Optional[Callable[[], float]] = None, *, grad_scale: Optional[torch.Tensor] = None) -> Optional[float]:
+        """One optimisation step.  ``closure`` is not supported and must be ``None``.
+
+        ``grad_scale``: one float32 value on the parameters' device that multiplies every gradient, such as the factor
+        of ``hip_kernels.global_grad_norm(grads, max_norm=...)``; the gradients themselves stay as they are.
+        """
+        if closure is not None:
+            raise ValueError("closure is not supported")
+        capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+        if capturing and not self.capturable:
+            raise RuntimeError("capturing AdamW.step() needs capturable=True")
+        for group in self.param_groups:
+            self._init_group(group)
+            batches: dict = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("AdamW does not support sparse gradients")
+                state = self.state[p]
+                if not self.capturable:
+                    state["step"] += 1
+                held = state.get("master", p)
+                if self._kernels_take(p, held):
+                    key = (p.device, p.dtype, p.grad.dtype, held is p, None if self.capturable else state["step"])
+                    batches.setdefault(key, []).append(p)
+                else:
+                    if self.capturable:
+                        state["step"] += 1
+                    self._update_torch(p, group, grad_scale)
+            for members in batches.values():
+                self._update_batch(members, group, grad_scale)
+        return None
+
+    @staticmethod
+    def _kernels_take(p: torch.Tensor, held: torch.Tensor) -> bool:
+        if not (hip_kernels.on_kernel_device(p) and p.dtype in DTYPE_CODES and p.grad.dtype in DTYPE_CODES):
+            return False
+        hip_kernels.require_library()
+        half = {torch.bfloat16, torch.float16}
+        return p.dtype not in half or p.grad.dtype not in half or p.dtype == p.grad.dtype
+
+    def _update_batch(self, members: list, group: dict, grad_scale: Optional[torch.Tensor]) -> None:
+        """One call for parameters of one device, type and step."""
+        states = [self.state[p] for p in members]
+        grads = [p.grad if p.grad.stride() == p.stride() else torch.empty_like(p, dtype=p.grad.dtype).copy_(p.grad) for p in members]
+        step: Any = states[0]["step"]
+        if self.capturable:
+            step = [s["step"] for s in states]
+            torch._foreach_add_(step, 1)
+        masters = "master" in states[0]
+        (hip_kernels.fused_adamw_update if self.moment_bits == 32 else hip_kernels.fused_adamw_update_8bit)(
+            [s["master"] for s in states] if masters else [p.detach() for p in members],
+            grads,
+            [s["exp_avg"] for s in states],
+            [s["exp_avg_sq"] for s in states],
+            step=step,
+            lr=group["lr"],
+            beta1=group["betas"][0],
+            beta2=group["betas"][1],
+            eps=group["eps"],
+            weight_decay=group["weight_decay"],
+            weight_decay_method=self.weight_decay_method,
+            grad_scale=grad_scale,
+            model_params=[p.detach() for p in members] if masters else None,
+        )
+
+    def _update_torch(self, p: torch.Tensor, group: dict, grad_scale: Optional[torch.Tensor]) -> None:
+        """The update of one parameter as torch statements, in float32 (float64 parameters: in float64)."""
+        state, lr, (beta1, beta2) = self.state[p], float(group["lr"]), group["betas"]
+        held = state.get("master", p)
+        wide = torch.promote_types(p.dtype, torch.float32)
+        w, grad = held.to(wide, copy=True), p.grad.to(wide, copy=True)
+        if grad_scale is not None:
+            grad.mul_(grad_scale)
+        self._apply_weight_decay_inplace(w, grad, lr, group["weight_decay"])
+        if self.moment_bits == 8:
+            m, v = (_unpack_torch(state[k], p.numel(), k).as_strided(w.shape, w.stride()) for k in ("exp_avg", "exp_avg_sq"))
+        else:
+            m, v = state["exp_avg"], state["exp_avg_sq"]
+        m.lerp_(grad, 1 - beta1)
+        v.mul_(beta2).addcmul_(grad, grad, value=1 - beta2)
+        t = state["step"]
+        den = (v / (1 - beta2**t)).sqrt_().add_(group["eps"])
+        w.sub_(lr / (1 - beta1**t) * (m / den))
+        if self.moment_bits == 8:
+            for k, x in (("exp_avg", m), ("exp_avg_sq", v)):
+                state[k].copy_(_pack_torch(_memory_order(x), k))
+        held.copy_(w)
+        if held is not p:
+            p.copy_(w)
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict: dict) -> None:
+        """Loads a checkpoint of this class or of ``torch.optim.AdamW``.  Moments come in either width and are held in
+        the one of this optimizer; a missing float32 copy of a 16-bit parameter is made from the parameter."""
+        super().load_state_dict(state_dict)
+        saved = state_dict["state"]
+        for group, saved_group in zip(self.param_groups, state_dict["param_groups"]):
+            for p, index in zip(group["params"], saved_group["params"]):
+                if index not in saved:
+                    continue
+                state = self.state[p]
+                # (the base class casts what it loads to the parameter's type)
+                state["exp_avg"], state["exp_avg_sq"] = (self._loaded_moment(saved[index][k], p, k) for k in ("exp_avg", "exp_avg_sq"))
+                step = float(saved[index]["step"])
+                state["step"] = self._first_step(p).fill_(step) if self.capturable else int(step)
+                if self.master_weights and p.dtype in (torch.bfloat16, torch.float16):
+                    state["master"] = saved[index].get("master", p.detach()).to(device=p.device, dtype=torch.float32, copy=True)
+                else:
+                    state.pop("master", None)
+
+    def _loaded_moment(self, value: torch.Tensor, p: torch.Tensor, which: str) -> torch.Tensor:
+        packed = value.dtype == torch.uint8 and value.dim() == 1
+        if packed and value.numel() != hip_kernels.moment_8bit_bytes(p.numel()):
+            raise ValueError(f"{which} of {value.numel()} bytes for a parameter of {p.numel()} values")
+        if packed and self.moment_bits == 8:
+            return value.to(p.device, copy=True)
+        new = self._moment(p)
+        kernels = hip_kernels.on_kernel_device(p)
+        if not packed:
+            wide = torch.empty_like(p, dtype=torch.promote_types(p.dtype, torch.float32)).copy_(value)
+            if self.moment_bits == 32:
+                return wide
+            if kernels:
+                hip_kernels.pack_moments_8bit([wide], [new], which=which)
+                return new
+            return new.copy_(_pack_torch(_memory_order(wide), which))
+        value = value.to(p.device)
+        if kernels and new.dtype == torch.float32:
+            hip_kernels.unpack_moments_8bit([value], [new], which=which)
+        else:
+            _memory_order(new).copy_(_unpack_torch(value, p.numel(), which))
+        return new

@@ -3,12 +3,15 @@
 from __future__ import annotations
 
 import contextlib
-from typing import Iterator, Literal
+from typing import Iterable, Iterator, Literal, Union
 
 import torch
 
+from emerging_optimizers import hip_kernels
+from emerging_optimizers.hip_kernels._launch import DTYPE_CODES, is_dense
 
-__all__ = ["fp32_matmul_precision", "FP32MatmulPrecT"]
+
+__all__ = ["clip_grad_norm_", "fp32_matmul_precision", "FP32MatmulPrecT"]
 
 FP32MatmulPrecT = Literal["highest", "high", "medium"]
 
@@ -26,3 +29,41 @@ def fp32_matmul_precision(precision: FP32MatmulPrecT = "highest") -> Iterator[No
         yield
     finally:
         torch.set_float32_matmul_precision(saved)
+
+
+@torch.no_grad()
+def clip_grad_norm_(
+    parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, *, error_if_nonfinite: bool = False
+) -> torch.Tensor:
+    """Scales the gradients of ``parameters`` in place so that their global 2-norm is at most ``max_norm``.
+
+    Same convention as ``torch.nn.utils.clip_grad_norm_`` (factor ``min(1, max_norm / (norm + 1e-6))``, the norm is
+    returned as a float32 scalar).  Gradients on one gfx950 GPU that fill their memory take two multi-tensor passes of the kernels
+    (``hip_kernels.clip_grads_by_global_norm``) and nothing waits for the GPU unless ``error_if_nonfinite`` asks for
+    the norm.
+    """
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm must not be negative, got {max_norm}")
+    if not grads:
+        return torch.tensor(0.0)
+    kernels = len({g.device for g in grads}) == 1 and all(
+        hip_kernels.on_kernel_device(g) and g.dtype in DTYPE_CODES and is_dense(g) for g in grads
+    )
+    if kernels and not error_if_nonfinite:
+        return hip_kernels.clip_grads_by_global_norm(grads, max_norm=max_norm)
+    if kernels:
+        norm, factor = hip_kernels.global_grad_norm(grads, max_norm=max_norm)
+    else:
+        norm = torch.stack([torch.linalg.vector_norm(g, dtype=torch.float64).to(grads[0].device) for g in grads]).square().sum().sqrt().float()
+        factor = (max_norm / (norm + 1e-6)).clamp(max=1.0)
+    if error_if_nonfinite and not bool(norm.isfinite()):
+        raise RuntimeError(f"The global 2-norm of the gradients is {float(norm)}")
+    if kernels:
+        hip_kernels.scale_tensors(grads, factor)
+    else:
+        for g in grads:
+            g.mul_(factor.to(g.device))
+    return norm

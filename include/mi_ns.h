@@ -1,6 +1,6 @@
 /*
- * mi_ns.h - C ABI of libmi_ns.so: bf16 SYRK, GEMM+AXPY, Frobenius normalisation and the
- * Newton-Schulz orthogonalisation driver for AMD MI355X (gfx950).
+ * mi_ns.h - C ABI of libmi_ns.so: bf16 SYRK, GEMM+AXPY, Frobenius normalisation, the
+ * Newton-Schulz orthogonalisation driver and multi-tensor AdamW for AMD MI355X (gfx950).
  *
  * The reference project (NVIDIA-NeMo/Emerging-Optimizers) is pure Python and has no FFI for this
  * path; each entry point below names the Python call site(s) of the reference that it stands
@@ -213,6 +213,74 @@ int mi_muon_update_bf16(float* param, const float* grad, float* momentum, int64_
                         float beta, int nesterov, float param_decay, float update_scale,
                         const float* abc, int steps, float eps, int accumulate_fp64,
                         void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Optimizer operators over lists of tensors, for the parameters that are not orthogonalised (embeddings, output head,
+ * gains, biases).  The reference leaves those to torch.optim.AdamW; there is no counterpart of these entries in it.
+ *
+ * A list is `count` device pointers in a HOST array, with the element counts in another; the arrays are read during the
+ * call only.  Tensors are contiguous, need the alignment of their elements only (8-bit moments: 16 bytes) and may have
+ * any size from 0 to 2^35 elements.  No tensor that a call writes may overlap another tensor of the call.  One launch
+ * serves up to 60 tensors (192 for the norm and the scaling, 128 for the conversions); nothing is allocated, copied
+ * or waited for, so calls may be captured into a HIP graph (with a step count on the device where it has to advance).
+ */
+#define MI_DTYPE_F32 0
+#define MI_DTYPE_BF16 1
+#define MI_DTYPE_F16 2
+
+/* Weight-decay methods (mixin.py:35-56 of the reference): what multiplies the weight, or joins the gradient. */
+#define MI_DECAY_DECOUPLED 0   /* param *= 1 - weight_decay * lr    */
+#define MI_DECAY_INDEPENDENT 1 /* param *= 1 - weight_decay         */
+#define MI_DECAY_L2 2          /* grad  += weight_decay * param     */
+#define MI_DECAY_PALM 3        /* param *= 1 - weight_decay * lr^2  */
+
+/*
+ * One AdamW step of every tensor of the list:
+ *   g <- grad_scale * grad (+ weight_decay * param);  m <- beta1 m + (1 - beta1) g;  v <- beta2 v + (1 - beta2) g^2
+ *   param <- keep * param - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * in float32, each result rounded to its type once.
+ *
+ * param: weights of record, float32, bfloat16 or float16 (param_dtype).  model_param: NULL, or 16-bit copies
+ * (model_dtype) of float32 weights, written only.  grad: float32, or the 16-bit type that the weights or their copies
+ * have (either one for float32 weights without copies).  exp_avg, exp_avg_sq: the moments m and v, updated in place;
+ * moment_bits == 32: float32 values; moment_bits == 8: the 8-bit form described at mi_moments_8bit_pack.
+ * t = step (>= 1), or, where step_dev is not NULL, *step_dev[i] for tensor i (float32 on the device).
+ * lr_dev: NULL, or a float32 on the device that replaces lr.  grad_scale: NULL (1), or a float32 on the device.
+ */
+int mi_adamw_update(int64_t count, void* const* param, const void* const* grad, void* const* exp_avg,
+                    void* const* exp_avg_sq, void* const* model_param, const float* const* step_dev,
+                    const int64_t* numel, int param_dtype, int grad_dtype, int model_dtype, int moment_bits,
+                    double step, double lr, const float* lr_dev, double beta1, double beta2, double eps,
+                    double weight_decay, int decay_method, const float* grad_scale, void* stream);
+
+/*
+ * Global 2-norm of a list: out[0] = sqrt(sum of all squares), out[1] = min(1, max_norm / (out[0] + 1e-6)) (float32 on
+ * the device).  Sums in float64 in a fixed order.  dtype: HOST array, one MI_DTYPE_* per tensor.  partials: float64
+ * device scratch of mi_global_norm_partials_len(count, numel) elements that no other call in flight uses.
+ */
+size_t mi_global_norm_partials_len(int64_t count, const int64_t* numel);
+int mi_global_norm(int64_t count, const void* const* x, const int64_t* numel, const int* dtype, double max_norm,
+                   double* partials, size_t partials_len, float* out, void* stream);
+
+/* x <- *factor * x for every tensor of the list (factor: float32 on the device; exactly 1 leaves everything alone). */
+int mi_scale_tensors(int64_t count, void* const* x, const int64_t* numel, const int* dtype, const float* factor,
+                     void* stream);
+
+/*
+ * 8-bit form of an AdamW moment.  n values are ceil(n / 64) blocks of 64; the form is one byte of code for each place
+ * of each block, then one float32 scale s for each block, mi_moment_8bit_bytes(n) bytes together.  s is the largest
+ * magnitude of the block.
+ *   first moment:  code k in -127 .. 127 stands for sign(k) s (k / 127)^2; |k| = round(127 sqrt(|m| / s))
+ *   second moment: code k in 0 .. 255 stands for s (k / 255)^4; k = round(255 (v / s)^(1/4)), at least 1 for v > 0
+ * A block with a value that is not finite stands for NaN throughout (s = NaN), one whose largest magnitude is below
+ * 2^-126 for 0; codes behind the last value are 0.  pack writes the form of float32, bfloat16 or float16 values
+ * (dtype), unpack the values that a form stands for.  second_moment: 0 or 1.
+ */
+size_t mi_moment_8bit_bytes(int64_t numel);
+int mi_moments_8bit_pack(int64_t count, const void* const* src, void* const* packed, const int64_t* numel, int dtype,
+                         int second_moment, void* stream);
+int mi_moments_8bit_unpack(int64_t count, const void* const* packed, void* const* dst, const int64_t* numel, int dtype,
+                           int second_moment, void* stream);
 
 /*
  * Per-kernel timing of mi_newton_schulz_bf16 for benchmarks (no counterpart in the reference, whose
