@@ -223,6 +223,64 @@ int selftest() {
 
 }  // namespace
 
+// Lists of tensors: sizes on both sides of vectors, blocks, chunks and launch limits, more tensors than an argument block
+// holds, sizes past 32 bits; every entry, every combination of types.
+void list_case(const std::vector<int64_t>& sizes, bool quick) {
+  const int64_t count = (int64_t)sizes.size();
+  const auto lists = [&](int bytes, const char* name) {
+    std::vector<void*> p;
+    for (int64_t n : sizes) p.push_back(n ? fake_alloc(bytes ? (size_t)n * bytes : mi_moment_8bit_bytes(n), name) : nullptr);
+    return p;
+  };
+  const auto bytes_of = [](int dtype) { return dtype == MI_DTYPE_F32 ? 4 : 2; };
+  const auto consts = [](const std::vector<void*>& p) { return const_cast<const void* const*>(p.data()); };
+  char what[100];
+  for (int bits : {32, 8})
+    for (int param = 0; param < 3; ++param)
+      for (int grad = 0; grad < 3; ++grad)
+        for (int low = -1; low < 3; ++low) {
+          if (low == 0 || (low > 0 && param != 0) || (quick && (param == 2 || grad == 2 || low == 2))) continue;
+          std::snprintf(what, sizeof what, "adamw %lld tensors from %lld, bits=%d types=%d %d %d", (long long)count, (long long)sizes[0], bits, param, grad, low);
+          begin(what);
+          const auto p = lists(bytes_of(param), "param"), g = lists(bytes_of(grad), "grad"), m = lists(bits == 8 ? 0 : 4, "exp_avg"),
+                     v = lists(bits == 8 ? 0 : 4, "exp_avg_sq"), l = lists(2, "copy");
+          const int rc = mi_adamw_update(count, p.data(), consts(g), m.data(), v.data(), low > 0 ? l.data() : nullptr, nullptr, sizes.data(), param, grad, low, bits, 1, 1e-3,
+                                         nullptr, 0.9, 0.95, 1e-8, 0.1, 0, nullptr, nullptr);
+          const int half = low > 0 ? low : param;
+          if (half && grad && half != grad) {
+            if (rc != MI_ERR_BAD_ARG) mi::host_check::fail("two 16-bit types were not refused");
+          } else {
+            expect_ok(rc);
+          }
+        }
+  for (int dtype = 0; dtype < 3; ++dtype) {
+    std::snprintf(what, sizeof what, "norm, clipping and conversions of %lld tensors from %lld, type %d", (long long)count, (long long)sizes[0], dtype);
+    begin(what);
+    const auto x = lists(bytes_of(dtype), "tensor"), q = lists(0, "8-bit form");
+    const std::vector<int> types(count, dtype);
+    const size_t len = mi_global_norm_partials_len(count, sizes.data());
+    double* partials = static_cast<double*>(fake_alloc(len * 8, "partials"));
+    float* out = static_cast<float*>(fake_alloc(8, "norm and factor"));
+    expect_ok(mi_global_norm(count, consts(x), sizes.data(), types.data(), 1.0, partials, len, out, nullptr));
+    expect_ok(mi_clip_by_global_norm(count, x.data(), sizes.data(), types.data(), 1.0, partials, len, out, nullptr));
+    expect_ok(mi_scale_tensors(count, x.data(), sizes.data(), types.data(), out, nullptr));
+    for (int second : {0, 1}) {
+      expect_ok(mi_moments_8bit_pack(count, consts(x), q.data(), sizes.data(), dtype, second, nullptr));
+      expect_ok(mi_moments_8bit_unpack(count, consts(q), x.data(), sizes.data(), dtype, second, nullptr));
+    }
+  }
+}
+void list_cases(bool quick) {
+  list_case({1}, quick);
+  list_case({0, 3, 4, 5, 63, 64, 65, 1023, 1024, 1025, 2047, 2048, 2049, 4095, 4097, 16383, 16384, 16385, 0}, quick);
+  std::vector<int64_t> many;
+  for (int64_t i = 0; i < 400; ++i) many.push_back(1 + i * 7919 % 5000);
+  list_case(many, quick);
+  const int64_t launch = (int64_t)1 << 33;  // 2^23 chunks of 1024 values
+  list_case({5, launch - 1024, 7, launch, launch + 1, 9, 3 * launch + 77, 11}, quick);
+  list_case({((int64_t)1 << 40) - 5}, quick);
+}
+
 int main(int argc, char** argv) {
   if (argc > 1 && std::strcmp(argv[1], "--selftest") == 0) return selftest();
   const bool quick = argc > 1 && std::strcmp(argv[1], "--quick") == 0;
@@ -231,6 +289,7 @@ int main(int argc, char** argv) {
   const bool bench_only = bench_exhaustive || (argc > 1 && std::strcmp(argv[1], "--bench") == 0);
   state().exhaustive = bench_exhaustive;
   validation_cases();
+  if (!bench_only) list_cases(quick);
   // ---- lower-triangle products
   const int64_t ns_[] = {256, 384, 512, 768, 1024, 1032, 1096, 1152, 1280, 1536, 1792, 1800, 2048, 2304, 3072, 4096, 5120, 8184, 8192};
   const int64_t ks_[] = {64, 128, 192, 448, 1024, 4096, 8192, 14336};

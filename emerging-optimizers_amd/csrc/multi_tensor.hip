@@ -21,9 +21,10 @@ namespace {
 
 constexpr int NT = 256;  // threads of a workgroup
 constexpr int BLOCK8 = 64;  // values that share a scale in the 8-bit form of a moment
-// A launch's workgroup count stays below 2^24 (2^32 threads) with room to spare; one tensor must fit into one launch.
+// A launch's workgroup count stays below 2^24 (2^32 threads) with room to spare; a tensor of more chunks takes several
+// launches.  Chunks of one tensor are numbered in 32 bits.
 constexpr int64_t MAX_CHUNKS = (int64_t)1 << 23;
-constexpr int64_t MAX_NUMEL = (int64_t)1 << 35;
+constexpr int64_t MAX_NUMEL = (int64_t)1 << 40;
 
 // ---------------------------------------------------------------------------------------------
 // Argument blocks (4 KB at most)
@@ -33,9 +34,11 @@ struct AdamTensor {
   const void* g;
   void* m;            // moments: float32 values, or the 8-bit form (codes, then the blocks' scales)
   void* v;
-  void* low;          // 16-bit copy of the updated weights, or null
   const float* step;  // device step counter, or null (the call's own)
   int64_t n;
+};
+struct AdamTensorCopy : AdamTensor {
+  void* low;  // 16-bit copy of the updated weights
 };
 struct AdamScalars {
   float b1, omb1, b2, omb2, eps, keep, l2, step_size, inv_sqrt_bc2;
@@ -51,13 +54,20 @@ struct TensorList {
   T t[N];
   uint32_t first[N];  // number of the tensor's first chunk
   int count;
+  uint32_t chunk0;  // number of the launch's first chunk
 };
-typedef TensorList<AdamTensor, 60> AdamList;
+struct None {};  // no 16-bit copies
+template <class LT>
 struct AdamArgs {
-  AdamList list;
+  TensorList<AdamTensorCopy, 66> list;
   AdamScalars s;
 };
-static_assert(sizeof(AdamArgs) <= 4096, "argument block");
+template <>
+struct AdamArgs<None> {
+  TensorList<AdamTensor, 76> list;
+  AdamScalars s;
+};
+static_assert(sizeof(AdamArgs<None>) <= 4096 && sizeof(AdamArgs<float>) <= 4096, "argument block");
 
 struct ReadTensor {
   const void* x;
@@ -85,35 +95,41 @@ __host__ __device__ __forceinline__ int tensor_of(const L& l, uint32_t b) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// Four values at a time.  Tensors need the alignment of their elements only: the vector types say so, and global
-// loads and stores of any width take such addresses.
+// V values at a time, 4 of float32 or 8 where all types have 16 bits (16 bytes a lane).  Tensors need the alignment of their elements only: the vector types say so, and global
+// loads and stores of any width take such addresses.  A step touches each value once and a list is far larger than the
+// caches, so loads and stores are non-temporal: 268M float32 weights with float32 moments 1395 -> 1294 us (5.4 -> 5.8 TB/s;
+// loads alone 1351, stores alone 1414), the sum of squares of as many values 182 -> 160 us (6.7 TB/s).
 // ---------------------------------------------------------------------------------------------
-template <class T>
-struct Quad {
-  typedef T type __attribute__((ext_vector_type(4)));
+template <class T, int V>
+struct Pack {
+  typedef T type __attribute__((ext_vector_type(V)));
   typedef type at __attribute__((aligned(sizeof(T))));
 };
-template <class T>
-__device__ __forceinline__ f32x4_t load4(const T* p) {
-  return __builtin_convertvector((typename Quad<T>::type)(*reinterpret_cast<const typename Quad<T>::at*>(p)), f32x4_t);
+template <int V>
+using Floats = typename Pack<float, V>::type;
+template <int V, class T>
+__device__ __forceinline__ Floats<V> load(const T* p) {
+  typedef Pack<T, V> X;
+  return __builtin_convertvector((typename X::type)__builtin_nontemporal_load(reinterpret_cast<const typename X::at*>(p)), Floats<V>);
 }
-template <class T>
-__device__ __forceinline__ void store4(T* p, f32x4_t x) {
-  *reinterpret_cast<typename Quad<T>::at*>(p) = __builtin_convertvector(x, typename Quad<T>::type);
+template <int V, class T>
+__device__ __forceinline__ void store(T* p, Floats<V> x) {
+  typedef Pack<T, V> X;
+  __builtin_nontemporal_store((typename X::at)__builtin_convertvector(x, typename X::type), reinterpret_cast<typename X::at*>(p));
 }
-// The first `k` of four values; zeros for the others.
-template <class T>
-__device__ __forceinline__ f32x4_t load4_part(const T* p, int k) {
-  f32x4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
+// The first `k` of V values; zeros for the others.
+template <int V, class T>
+__device__ __forceinline__ Floats<V> load_part(const T* p, int k) {
+  Floats<V> x = {};
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < V; ++i)
     if (i < k) x[i] = (float)p[i];
   return x;
 }
-template <class T>
-__device__ __forceinline__ void store4_part(T* p, f32x4_t x, int k) {
+template <int V, class T>
+__device__ __forceinline__ void store_part(T* p, Floats<V> x, int k) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < V; ++i)
     if (i < k) p[i] = (T)x[i];
 }
 
@@ -150,78 +166,74 @@ __device__ __forceinline__ AdamCoef adam_coefficients(const AdamScalars& s, cons
 }
 
 // m <- b1 m + (1 - b1) g,  v <- b2 v + (1 - b2) g^2,  p <- keep p - step_size m / (sqrt(v) inv_sqrt_bc2 + eps)
+//
+// FAST: square root and reciprocal of the hardware, each within one unit in the last place, for which a number below the
+// smallest normal one is 0.  The correctly rounded sequences cost about 25 instructions a value: nothing beside 32-bit
+// moments, where the memory sets the pace, and twice the time beside 8-bit ones (see below).
+template <bool FAST>
 __device__ __forceinline__ void adam_value(float& p, float g, float& m, float& v, const AdamCoef& c) {
   g *= c.gscale;
   if (c.l2 != 0.0f) g = fmaf(c.l2, p, g);
   m = fmaf(c.b1, m, c.omb1 * g);
   v = fmaf(c.b2, v, c.omb2 * g * g);
-  const float den = fmaf(sqrtf(v), c.inv_sqrt_bc2, c.eps);
-  p = fmaf(-c.step_size, m / den, c.keep * p);
+  const float den = fmaf(FAST ? __builtin_amdgcn_sqrtf(v) : sqrtf(v), c.inv_sqrt_bc2, c.eps);
+  p = fmaf(-c.step_size, FAST ? m * __builtin_amdgcn_rcpf(den) : m / den, c.keep * p);
 }
 
 // 32-bit moments.  Each value is read and written once: 28 bytes a value with float32 weights and gradients, about 25
 // operations, so the memory bounds it.
-constexpr int ADAM_U = 4;
-constexpr int ADAM_CHUNK = NT * 4 * ADAM_U;
-
-struct None {};
+constexpr int ADAM_V = 4, ADAM_U = 1;
+constexpr int ADAM_CHUNK = NT * ADAM_V * ADAM_U;
 
 template <class PT, class GT, class LT>
-__global__ __launch_bounds__(NT) void adamw_kernel(AdamArgs a) {
-  const int ti = tensor_of(a.list, blockIdx.x);
-  const AdamTensor t = a.list.t[ti];
-  const int64_t base = (int64_t)(blockIdx.x - a.list.first[ti]) * ADAM_CHUNK;
+__global__ __launch_bounds__(NT) void adamw_kernel(AdamArgs<LT> a) {
+  constexpr int V = ADAM_V;
+  typedef Floats<V> F;
+  const uint32_t chunk = a.list.chunk0 + blockIdx.x;
+  const int ti = tensor_of(a.list, chunk);
+  const auto t = a.list.t[ti];
+  const int64_t base = (int64_t)(chunk - a.list.first[ti]) * ADAM_CHUNK;
   PT* __restrict__ p = static_cast<PT*>(t.p) + base;
   const GT* __restrict__ g = static_cast<const GT*>(t.g) + base;
   float* __restrict__ m = static_cast<float*>(t.m) + base;
   float* __restrict__ v = static_cast<float*>(t.v) + base;
   const int64_t left = t.n - base;
   const AdamCoef c = adam_coefficients(a.s, t.step);
-  if (left >= ADAM_CHUNK) {
-    f32x4_t pp[ADAM_U], gg[ADAM_U], mm[ADAM_U], vv[ADAM_U];
-#pragma unroll
-    for (int u = 0; u < ADAM_U; ++u) {
-      const int e = (u * NT + threadIdx.x) * 4;
-      gg[u] = load4(g + e);
-      pp[u] = load4(p + e);
-      mm[u] = load4(m + e);
-      vv[u] = load4(v + e);
-    }
-#pragma unroll
-    for (int u = 0; u < ADAM_U; ++u) {
-      const int e = (u * NT + threadIdx.x) * 4;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float pi = pp[u][i], mi = mm[u][i], vi = vv[u][i];
-        adam_value(pi, gg[u][i], mi, vi, c);
-        pp[u][i] = pi;
-        mm[u][i] = mi;
-        vv[u][i] = vi;
-      }
-      store4(p + e, pp[u]);
-      store4(m + e, mm[u]);
-      store4(v + e, vv[u]);
-      if constexpr (!__is_same(LT, None)) store4(static_cast<LT*>(t.low) + base + e, pp[u]);
-    }
-    return;
-  }
   for (int u = 0; u < ADAM_U; ++u) {
-    const int e = (u * NT + threadIdx.x) * 4;
+    const int e = (u * NT + threadIdx.x) * V;
     if (e >= left) return;
-    const int k = left - e < 4 ? (int)(left - e) : 4;
-    f32x4_t pp = load4_part(p + e, k), gg = load4_part(g + e, k), mm = load4_part(m + e, k), vv = load4_part(v + e, k);
+    const int k = left - e < V ? (int)(left - e) : V;
+    F pp, gg, mm, vv;
+    if (k == V) {
+      gg = load<V>(g + e);
+      pp = load<V>(p + e);
+      mm = load<V>(m + e);
+      vv = load<V>(v + e);
+    } else {
+      gg = load_part<V>(g + e, k);
+      pp = load_part<V>(p + e, k);
+      mm = load_part<V>(m + e, k);
+      vv = load_part<V>(v + e, k);
+    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < V; ++i) {
       float pi = pp[i], mi = mm[i], vi = vv[i];
-      adam_value(pi, gg[i], mi, vi, c);
+      adam_value<false>(pi, gg[i], mi, vi, c);
       pp[i] = pi;
       mm[i] = mi;
       vv[i] = vi;
     }
-    store4_part(p + e, pp, k);
-    store4_part(m + e, mm, k);
-    store4_part(v + e, vv, k);
-    if constexpr (!__is_same(LT, None)) store4_part(static_cast<LT*>(t.low) + base + e, pp, k);
+    if (k == V) {
+      store<V>(p + e, pp);
+      store<V>(m + e, mm);
+      store<V>(v + e, vv);
+      if constexpr (!__is_same(LT, None)) store<V>(static_cast<LT*>(t.low) + base + e, pp);
+    } else {
+      store_part<V>(p + e, pp, k);
+      store_part<V>(m + e, mm, k);
+      store_part<V>(v + e, vv, k);
+      if constexpr (!__is_same(LT, None)) store_part<V>(static_cast<LT*>(t.low) + base + e, pp, k);
+    }
   }
 }
 
@@ -238,174 +250,212 @@ __global__ __launch_bounds__(NT) void adamw_kernel(AdamArgs a) {
 // ---------------------------------------------------------------------------------------------
 __host__ __device__ inline int64_t blocks8(int64_t n) { return (n + BLOCK8 - 1) / BLOCK8; }
 
-// Maximum over the 16 lanes of a row (a block is 16 lanes of 4 values): exchanges inside the row only, so every lane
-// of the row must be active.
-__device__ __forceinline__ uint32_t row_max(uint32_t x) {
+// Maximum over the lanes that hold a block: 16 with 4 values each, 8 with 8 (exchanges inside a row of 16 lanes; every
+// lane of the block must be active).
+template <int V>
+__device__ __forceinline__ uint32_t block_max(uint32_t x) {
+  static_assert(V == 4 || V == 8, "lanes of a block");
 #define MI_ROW_STEP(ctrl) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, 0xf, 0xf, true))
   MI_ROW_STEP(0xB1);   // quad_perm [1, 0, 3, 2]
   MI_ROW_STEP(0x4E);   // quad_perm [2, 3, 0, 1]
   MI_ROW_STEP(0x141);  // row_half_mirror: the other quad of eight lanes
-  MI_ROW_STEP(0x140);  // row_mirror: the other half of the row
+  if (V == 4) MI_ROW_STEP(0x140);  // row_mirror: the other half of the row
 #undef MI_ROW_STEP
   return x;
 }
 
-// Scale of the block this lane's four magnitudes belong to.  The bit patterns of magnitudes order as the numbers do,
-// with infinities and then NaN above every finite one.
-__device__ __forceinline__ float block_scale(f32x4_t x) {
+// Scale of the block this lane's magnitudes belong to.  The bit patterns of magnitudes order as the numbers do, with
+// infinities and then NaN above every finite one.
+template <int V>
+__device__ __forceinline__ float block_scale(Floats<V> x) {
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-  top = row_max(top);
+  for (int i = 0; i < V; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  top = block_max<V>(top);
   return top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : top < 0x00800000u ? 0.0f : __uint_as_float(top);
 }
 
-template <bool SIGNED>
-__device__ __forceinline__ uint32_t encode4(f32x4_t x, float s) {
-  uint32_t codes = 0;
-  const bool held = s > 0.0f;  // not for 0 and not for NaN
+template <int V>
+using Codes = typename Pack<uint32_t, V / 4>::type;
+
+// Codes of V values.  The product with 127 or 255 and the rounding to the nearest integer are one operation: the sum
+// with 1.5 * 2^23 leaves the integer (two's complement for negative ones) in the lowest byte.  With the hardware's roots
+// and reciprocal, a step of 268M bfloat16 weights with 8-bit moments takes 505 us instead of 875 with correctly rounded
+// ones and a conversion to int.
+template <int V, bool SIGNED>
+__device__ __forceinline__ Codes<V> encode(Floats<V> x, float s) {
+  float inv = s > 0.0f ? __builtin_amdgcn_rcpf(s) : 0.0f;  // (neither for 0 nor for NaN)
+  if (__builtin_expect(s > 0x1p125f, 0)) inv = 1.0f / s;   // below the smallest normal number, which v_rcp_f32 makes 0
+  const uint32_t least = s > 0.0f ? 1u : 0u;
+  uint32_t k[V];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float share = held ? fabsf(x[i]) / s : 0.0f;
+  for (int i = 0; i < V; ++i) {
+    const float root = __builtin_amdgcn_sqrtf(fabsf(x[i]) * inv);
     if constexpr (SIGNED) {
-      int k = (int)rintf(sqrtf(share) * 127.0f);
-      if (x[i] < 0.0f) k = -k;
-      codes |= ((uint32_t)k & 0xffu) << (8 * i);
+      k[i] = __float_as_uint(fmaf(copysignf(root, x[i]), 127.0f, 12582912.0f));
     } else {
-      uint32_t k = (uint32_t)rintf(sqrtf(sqrtf(share)) * 255.0f);
-      if (held && x[i] > 0.0f) k = max(k, 1u);
-      codes |= (k & 0xffu) << (8 * i);
+      k[i] = __float_as_uint(fmaf(__builtin_amdgcn_sqrtf(root), 255.0f, 12582912.0f));
+      k[i] = max(k[i], 0x4B400000u | min(__float_as_uint(x[i]), least));  // 1 at least for a value over 0
     }
   }
+  Codes<V> codes;
+#pragma unroll
+  for (int i = 0; i < V; i += 4)
+    codes[i / 4] = __builtin_amdgcn_perm(k[i + 1], k[i], 0x0c0c0400u) | __builtin_amdgcn_perm(k[i + 3], k[i + 2], 0x04000c0cu);
   return codes;
 }
-template <bool SIGNED>
-__device__ __forceinline__ f32x4_t decode4(uint32_t codes, float s) {
-  f32x4_t x;
+template <int V, bool SIGNED>
+__device__ __forceinline__ Floats<V> decode(Codes<V> codes, float s) {
+  Floats<V> x;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < V; ++i) {
     // the scale comes last: a share of it that is taken first would be denormal for scales far above the smallest number
     if constexpr (SIGNED) {
-      const float k = (float)(int8_t)(codes >> (8 * i));
+      const float k = (float)(int8_t)(codes[i / 4] >> (8 * (i % 4)));
       x[i] = k * fabsf(k) * (1.0f / (127 * 127)) * s;
     } else {
-      const float k = (float)((codes >> (8 * i)) & 0xffu);
+      const float k = (float)((codes[i / 4] >> (8 * (i % 4))) & 0xffu);
       const float k2 = k * k * (1.0f / (255 * 255));
       x[i] = k2 * k2 * s;
     }
   }
   return x;
 }
+template <int V>
+__device__ __forceinline__ Codes<V> load_codes(const uint8_t* p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const Codes<V>*>(p));
+}
+template <int V>
+__device__ __forceinline__ void store_codes(uint8_t* p, Codes<V> codes) {
+  __builtin_nontemporal_store(codes, reinterpret_cast<Codes<V>*>(p));
+}
 
-constexpr int ADAM8_U = 4;
-constexpr int ADAM8_CHUNK = NT * 4 * ADAM8_U;
-static_assert(ADAM8_CHUNK % BLOCK8 == 0, "chunks are whole blocks");
+template <class PT, class GT>
+struct Adam8Shape {
+  static constexpr int V = sizeof(PT) == 2 && sizeof(GT) == 2 ? 8 : 4, U = 1;
+  static constexpr int CHUNK = NT * V * U;
+};
 
 template <class PT, class GT, class LT>
-__global__ __launch_bounds__(NT) void adamw8_kernel(AdamArgs a) {
-  const int ti = tensor_of(a.list, blockIdx.x);
-  const AdamTensor t = a.list.t[ti];
-  const int64_t base = (int64_t)(blockIdx.x - a.list.first[ti]) * ADAM8_CHUNK;
+__global__ __launch_bounds__(NT) void adamw8_kernel(AdamArgs<LT> a) {
+  typedef Adam8Shape<PT, GT> S;
+  constexpr int V = S::V;
+  typedef Floats<V> F;
+  const uint32_t chunk = a.list.chunk0 + blockIdx.x;
+  const int ti = tensor_of(a.list, chunk);
+  const auto t = a.list.t[ti];
+  const int64_t base = (int64_t)(chunk - a.list.first[ti]) * S::CHUNK;
   PT* __restrict__ p = static_cast<PT*>(t.p) + base;
   const GT* __restrict__ g = static_cast<const GT*>(t.g) + base;
   const int64_t nb = blocks8(t.n);
-  uint8_t* m8 = static_cast<uint8_t*>(t.m);
-  uint8_t* v8 = static_cast<uint8_t*>(t.v);
-  uint32_t* __restrict__ mc = reinterpret_cast<uint32_t*>(m8 + base);
-  uint32_t* __restrict__ vc = reinterpret_cast<uint32_t*>(v8 + base);
-  float* __restrict__ ms = reinterpret_cast<float*>(m8 + nb * BLOCK8) + base / BLOCK8;
-  float* __restrict__ vs = reinterpret_cast<float*>(v8 + nb * BLOCK8) + base / BLOCK8;
+  uint8_t* __restrict__ mc = static_cast<uint8_t*>(t.m) + base;
+  uint8_t* __restrict__ vc = static_cast<uint8_t*>(t.v) + base;
+  float* __restrict__ ms = reinterpret_cast<float*>(static_cast<uint8_t*>(t.m) + nb * BLOCK8) + base / BLOCK8;
+  float* __restrict__ vs = reinterpret_cast<float*>(static_cast<uint8_t*>(t.v) + nb * BLOCK8) + base / BLOCK8;
   const int64_t left = t.n - base;
   const AdamCoef c = adam_coefficients(a.s, t.step);
-  for (int u = 0; u < ADAM8_U; ++u) {
-    const int e = (u * NT + threadIdx.x) * 4;
+  for (int u = 0; u < S::U; ++u) {
+    const int e = (u * NT + threadIdx.x) * V;
     const int b = e / BLOCK8;
-    if ((int64_t)b * BLOCK8 >= left) return;  // the whole row of 16 lanes, whose block this is
-    const int k = left - e >= 4 ? 4 : left - e > 0 ? (int)(left - e) : 0;
-    f32x4_t pp, gg;
-    if (k == 4) {
-      pp = load4(p + e);
-      gg = load4(g + e);
+    if ((int64_t)b * BLOCK8 >= left) return;  // all lanes of the block together
+    const int k = left - e >= V ? V : left - e > 0 ? (int)(left - e) : 0;
+    F pp, gg;
+    if (k == V) {
+      pp = load<V>(p + e);
+      gg = load<V>(g + e);
     } else {
-      pp = load4_part(p + e, k);
-      gg = load4_part(g + e, k);
+      pp = load_part<V>(p + e, k);
+      gg = load_part<V>(g + e, k);
     }
-    f32x4_t mm = decode4<true>(mc[e / 4], ms[b]), vv = decode4<false>(vc[e / 4], vs[b]);
+    F mm = decode<V, true>(load_codes<V>(mc + e), ms[b]), vv = decode<V, false>(load_codes<V>(vc + e), vs[b]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < V; ++i) {
       float pi = pp[i], mi = mm[i], vi = vv[i];
-      adam_value(pi, gg[i], mi, vi, c);
+      adam_value<true>(pi, gg[i], mi, vi, c);
       pp[i] = pi;
-      mm[i] = i < k ? mi : 0.0f;  // places behind the last value hold 0
-      vv[i] = i < k ? vi : 0.0f;
+      mm[i] = mi;
+      vv[i] = vi;
     }
-    const float sm = block_scale(mm), sv = block_scale(vv);
-    mc[e / 4] = encode4<true>(mm, sm);
-    vc[e / 4] = encode4<false>(vv, sv);
-    if ((threadIdx.x & 15) == 0) {
+    if (k < V) {  // places behind the last value hold 0
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i >= k) mm[i] = vv[i] = 0.0f;
+    }
+    const float sm = block_scale<V>(mm), sv = block_scale<V>(vv);
+    store_codes<V>(mc + e, encode<V, true>(mm, sm));
+    store_codes<V>(vc + e, encode<V, false>(vv, sv));
+    if (e % BLOCK8 == 0) {
       ms[b] = sm;
       vs[b] = sv;
     }
-    if (k == 4) {
-      store4(p + e, pp);
-      if constexpr (!__is_same(LT, None)) store4(static_cast<LT*>(t.low) + base + e, pp);
+    if (k == V) {
+      store<V>(p + e, pp);
+      if constexpr (!__is_same(LT, None)) store<V>(static_cast<LT*>(t.low) + base + e, pp);
     } else {
-      store4_part(p + e, pp, k);
-      if constexpr (!__is_same(LT, None)) store4_part(static_cast<LT*>(t.low) + base + e, pp, k);
+      store_part<V>(p + e, pp, k);
+      if constexpr (!__is_same(LT, None)) store_part<V>(static_cast<LT*>(t.low) + base + e, pp, k);
     }
   }
 }
 
 // Conversions between a list of tensors and their 8-bit forms.
-constexpr int MOVE_U = 4;
-constexpr int MOVE_CHUNK = NT * 4 * MOVE_U;
+template <class T>
+struct MoveShape {
+  static constexpr int V = sizeof(T) == 2 ? 8 : 4, U = 2;
+  static constexpr int CHUNK = NT * V * U;
+};
 
 template <class T, bool SIGNED>
 __global__ __launch_bounds__(NT) void pack8_kernel(MoveList l) {
-  const int ti = tensor_of(l, blockIdx.x);
+  typedef MoveShape<T> S;
+  constexpr int V = S::V;
+  const uint32_t chunk = l.chunk0 + blockIdx.x;
+  const int ti = tensor_of(l, chunk);
   const MoveTensor t = l.t[ti];
-  const int64_t base = (int64_t)(blockIdx.x - l.first[ti]) * MOVE_CHUNK;
+  const int64_t base = (int64_t)(chunk - l.first[ti]) * S::CHUNK;
   const T* __restrict__ x = static_cast<const T*>(t.src) + base;
-  uint8_t* out = static_cast<uint8_t*>(t.dst);
-  uint32_t* __restrict__ codes = reinterpret_cast<uint32_t*>(out + base);
-  float* __restrict__ scales = reinterpret_cast<float*>(out + blocks8(t.n) * BLOCK8) + base / BLOCK8;
+  uint8_t* __restrict__ codes = static_cast<uint8_t*>(t.dst) + base;
+  float* __restrict__ scales = reinterpret_cast<float*>(static_cast<uint8_t*>(t.dst) + blocks8(t.n) * BLOCK8) + base / BLOCK8;
   const int64_t left = t.n - base;
-  for (int u = 0; u < MOVE_U; ++u) {
-    const int e = (u * NT + threadIdx.x) * 4;
+#pragma unroll
+  for (int u = 0; u < S::U; ++u) {
+    const int e = (u * NT + threadIdx.x) * V;
     const int b = e / BLOCK8;
-    if ((int64_t)b * BLOCK8 >= left) return;  // the whole row of 16 lanes, whose block this is
-    const int k = left - e >= 4 ? 4 : left - e > 0 ? (int)(left - e) : 0;
-    const f32x4_t xx = k == 4 ? load4(x + e) : load4_part(x + e, k);
-    const float s = block_scale(xx);
-    codes[e / 4] = encode4<SIGNED>(xx, s);
-    if ((threadIdx.x & 15) == 0) scales[b] = s;
+    if ((int64_t)b * BLOCK8 >= left) return;  // all lanes of the block together
+    const int k = left - e >= V ? V : left - e > 0 ? (int)(left - e) : 0;
+    const Floats<V> xx = k == V ? load<V>(x + e) : load_part<V>(x + e, k);
+    const float s = block_scale<V>(xx);
+    store_codes<V>(codes + e, encode<V, SIGNED>(xx, s));
+    if (e % BLOCK8 == 0) scales[b] = s;
   }
 }
 
 template <class T, bool SIGNED>
 __global__ __launch_bounds__(NT) void unpack8_kernel(MoveList l) {
-  const int ti = tensor_of(l, blockIdx.x);
+  typedef MoveShape<T> S;
+  constexpr int V = S::V;
+  const uint32_t chunk = l.chunk0 + blockIdx.x;
+  const int ti = tensor_of(l, chunk);
   const MoveTensor t = l.t[ti];
-  const int64_t base = (int64_t)(blockIdx.x - l.first[ti]) * MOVE_CHUNK;
-  const uint8_t* in = static_cast<const uint8_t*>(t.src);
-  const uint32_t* __restrict__ codes = reinterpret_cast<const uint32_t*>(in + base);
-  const float* __restrict__ scales = reinterpret_cast<const float*>(in + blocks8(t.n) * BLOCK8) + base / BLOCK8;
+  const int64_t base = (int64_t)(chunk - l.first[ti]) * S::CHUNK;
+  const uint8_t* __restrict__ codes = static_cast<const uint8_t*>(t.src) + base;
+  const float* __restrict__ scales = reinterpret_cast<const float*>(static_cast<const uint8_t*>(t.src) + blocks8(t.n) * BLOCK8) + base / BLOCK8;
   T* __restrict__ x = static_cast<T*>(t.dst) + base;
   const int64_t left = t.n - base;
-  for (int u = 0; u < MOVE_U; ++u) {
-    const int e = (u * NT + threadIdx.x) * 4;
+#pragma unroll
+  for (int u = 0; u < S::U; ++u) {
+    const int e = (u * NT + threadIdx.x) * V;
     if (e >= left) return;
-    const f32x4_t xx = decode4<SIGNED>(codes[e / 4], scales[e / BLOCK8]);
-    if (left - e >= 4) store4(x + e, xx);
-    else store4_part(x + e, xx, (int)(left - e));
+    const Floats<V> xx = decode<V, SIGNED>(load_codes<V>(codes + e), scales[e / BLOCK8]);
+    if (left - e >= V) store<V>(x + e, xx);
+    else store_part<V>(x + e, xx, (int)(left - e));
   }
 }
 
 // ---------------------------------------------------------------------------------------------
 // Global norm and scaling
 // ---------------------------------------------------------------------------------------------
-constexpr int NORM_U = 16;
-constexpr int NORM_CHUNK = NT * 4 * NORM_U;
+constexpr int NORM_CHUNK = NT * 64;
 
 __device__ __forceinline__ double wave_sum(double x) {
 #pragma unroll
@@ -429,66 +479,115 @@ __device__ __forceinline__ double group_sum(double x) {
 // a whole model lose nothing.
 template <class T>
 __global__ __launch_bounds__(NT) void sumsq_list_kernel(ReadList l, double* __restrict__ partials) {
-  const int ti = tensor_of(l, blockIdx.x);
-  const int64_t base = (int64_t)(blockIdx.x - l.first[ti]) * NORM_CHUNK;
+  const uint32_t chunk = l.chunk0 + blockIdx.x;
+  const int ti = tensor_of(l, chunk);
+  const int64_t base = (int64_t)(chunk - l.first[ti]) * NORM_CHUNK;
   const T* __restrict__ x = static_cast<const T*>(l.t[ti].x) + base;
   const int64_t left = l.t[ti].n - base;
+  constexpr int V = 16 / sizeof(T);
   double sum = 0.0;
   if (left >= NORM_CHUNK) {
 #pragma unroll 4
-    for (int u = 0; u < NORM_U; ++u) {
-      const f32x4_t xx = load4(x + (u * NT + threadIdx.x) * 4);
+    for (int e = threadIdx.x * V; e < NORM_CHUNK; e += NT * V) {
+      const Floats<V> xx = load<V>(x + e);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum = fma((double)xx[i], (double)xx[i], sum);
+      for (int i = 0; i < V; ++i) sum = fma((double)xx[i], (double)xx[i], sum);
     }
   } else {
-    for (int64_t e = threadIdx.x * 4; e < left; e += NT * 4) {
-      const f32x4_t xx = load4_part(x + e, left - e < 4 ? (int)(left - e) : 4);
+    for (int64_t e = threadIdx.x * V; e < left; e += NT * V) {
+      const Floats<V> xx = left - e >= V ? load<V>(x + e) : load_part<V>(x + e, (int)(left - e));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum = fma((double)xx[i], (double)xx[i], sum);
+      for (int i = 0; i < V; ++i) sum = fma((double)xx[i], (double)xx[i], sum);
     }
   }
   sum = group_sum<NT>(sum);
   if (threadIdx.x == 0) partials[blockIdx.x] = sum;
 }
 
-// out[0] = norm, out[1] = min(1, max_norm / (norm + 1e-6)); a norm that is not a number makes the factor NaN.
-__global__ __launch_bounds__(1024) void norm_finish_kernel(const double* __restrict__ partials, int64_t count, float max_norm,
-                                                           float* __restrict__ out) {
+// A norm and the factor that clips to max_norm: min(1, max_norm / (norm + 1e-6)), NaN for a norm that is not a number.
+struct NormAndFactor {
+  float norm, factor;
+};
+__device__ __forceinline__ NormAndFactor norm_and_factor(double sum, float max_norm) {
+  const float norm = (float)sqrt(sum);
+  const float f = max_norm / (norm + 1e-6f);
+  return {norm, f > 1.0f ? 1.0f : f};
+}
+
+// Sum of all partial sums, in thread 0.  The order depends on THREADS: a call with up to FEW_PARTIALS of them adds them
+// up with NT threads, whoever does it.
+constexpr int64_t FEW_PARTIALS = 2 * NT;
+template <int THREADS>
+__device__ __forceinline__ double sum_partials(const double* __restrict__ partials, int64_t count) {
   double sum = 0.0;
-  for (int64_t i = threadIdx.x; i < count; i += 1024) sum += partials[i];
-  sum = group_sum<1024>(sum);
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < count; i += THREADS) sum += partials[i];
+  return group_sum<THREADS>(sum);
+}
+
+// out[0] = norm, out[1] = factor
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void norm_finish_kernel(const double* __restrict__ partials, int64_t count, float max_norm,
+                                                              float* __restrict__ out) {
+  const double sum = sum_partials<THREADS>(partials, count);
   if (threadIdx.x == 0) {
-    const float norm = (float)sqrt(sum);
-    out[0] = norm;
-    const float f = max_norm / (norm + 1e-6f);
-    out[1] = f > 1.0f ? 1.0f : f;
+    const NormAndFactor r = norm_and_factor(sum, max_norm);
+    out[0] = r.norm;
+    out[1] = r.factor;
   }
 }
 
-constexpr int SCALE_U = 4;
-constexpr int SCALE_CHUNK = NT * 4 * SCALE_U;
-
-// x <- factor x; a factor of 1 changes nothing and reads nothing.
 template <class T>
-__global__ __launch_bounds__(NT) void scale_list_kernel(ReadList l, const float* __restrict__ factor) {
-  const float f = *factor;
+struct ScaleShape {
+  static constexpr int V = 16 / sizeof(T), U = 1;
+  static constexpr int CHUNK = NT * V * U;
+};
+
+// x <- factor x; a factor of 1 changes nothing and reads nothing.  The factor is *factor, or, with FINISH, what the
+// partial sums of a norm give: with few of them every workgroup adds them up itself (they come out of the cache), the
+// first one stores norm and factor, and clipping takes two launches instead of three.
+struct ScaleFactor {
+  const float* factor;
+  const double* partials;
+  int64_t count;
+  float max_norm;
+  float* out;
+};
+
+template <class T, bool FINISH>
+__global__ __launch_bounds__(NT) void scale_list_kernel(ReadList l, ScaleFactor sf) {
+  typedef ScaleShape<T> S;
+  constexpr int V = S::V;
+  float f;
+  if constexpr (FINISH) {
+    __shared__ float shared_factor;
+    const double sum = sum_partials<NT>(sf.partials, sf.count);
+    if (threadIdx.x == 0) {
+      const NormAndFactor r = norm_and_factor(sum, sf.max_norm);
+      shared_factor = r.factor;
+      if (blockIdx.x == 0) {
+        sf.out[0] = r.norm;
+        sf.out[1] = r.factor;
+      }
+    }
+    __syncthreads();
+    f = shared_factor;
+  } else {
+    f = *sf.factor;
+  }
   if (f == 1.0f) return;
-  const int ti = tensor_of(l, blockIdx.x);
-  const int64_t base = (int64_t)(blockIdx.x - l.first[ti]) * SCALE_CHUNK;
+  const uint32_t chunk = l.chunk0 + blockIdx.x;
+  const int ti = tensor_of(l, chunk);
+  const int64_t base = (int64_t)(chunk - l.first[ti]) * S::CHUNK;
   T* __restrict__ x = static_cast<T*>(const_cast<void*>(l.t[ti].x)) + base;
   const int64_t left = l.t[ti].n - base;
-  if (left >= SCALE_CHUNK) {
-    f32x4_t xx[SCALE_U];
 #pragma unroll
-    for (int u = 0; u < SCALE_U; ++u) xx[u] = load4(x + (u * NT + threadIdx.x) * 4);
-#pragma unroll
-    for (int u = 0; u < SCALE_U; ++u) store4(x + (u * NT + threadIdx.x) * 4, xx[u] * f);
-    return;
-  }
-  for (int64_t e = threadIdx.x * 4; e < left; e += NT * 4) {
-    const int k = left - e < 4 ? (int)(left - e) : 4;
-    store4_part(x + e, load4_part(x + e, k) * f, k);
+  for (int u = 0; u < S::U; ++u) {
+    const int e = (u * NT + threadIdx.x) * V;
+    if (e >= left) return;
+    const int k = (int)(left - e);
+    if (left - e >= V) store<V>(x + e, load<V>(x + e) * f);
+    else store_part<V>(x + e, load_part<V>(x + e, k) * f, k);
   }
 }
 
@@ -496,11 +595,13 @@ __global__ __launch_bounds__(NT) void scale_list_kernel(ReadList l, const float*
 // Host side
 // ---------------------------------------------------------------------------------------------
 // Walks a list of tensors and hands full argument blocks to `launch(list, chunks)`: empty tensors are left out, a block
-// ends when it is full or its chunks would be too many.  `fill(i)` makes the entry of tensor i.
+// ends when it is full or its chunks would be too many, and a tensor with too many of them has launches of its own.
+// `fill(i)` makes the entry of tensor i.
 template <class L, class Fill, class Launch>
 int for_each_list(int64_t count, const int64_t* numel, int64_t chunk, L& list, Fill fill, Launch launch) {
   int64_t chunks = 0;
   list.count = 0;
+  list.chunk0 = 0;
   for (int64_t i = 0; i < count; ++i) {
     if (numel[i] == 0) continue;
     const int64_t c = (numel[i] + chunk - 1) / chunk;
@@ -512,6 +613,15 @@ int for_each_list(int64_t count, const int64_t* numel, int64_t chunk, L& list, F
     list.first[list.count] = (uint32_t)chunks;
     list.t[list.count++] = fill(i);
     chunks += c;
+    if (chunks > MAX_CHUNKS) {
+      for (int64_t at = 0; at < c; at += MAX_CHUNKS) {
+        list.chunk0 = (uint32_t)at;
+        if (int rc = launch(list, std::min(MAX_CHUNKS, c - at))) return rc;
+      }
+      list.count = 0;
+      list.chunk0 = 0;
+      chunks = 0;
+    }
   }
   return list.count ? launch(list, chunks) : MI_OK;
 }
@@ -525,8 +635,10 @@ int launched(const char* who) {
 // Every chunk of a launch falls into the tensor the bisection finds, at an offset inside it.
 template <class L>
 void walk(const L& l, int64_t chunks, int64_t chunk) {
-  for (int64_t b = 0; b < chunks; b += (chunks > 4096 && b > 64 && b < chunks - 64) ? 61 : 1) {
+  for (int64_t i = 0; i < chunks; i += (chunks > 4096 && i > 64 && i < chunks - 64) ? 61 : 1) {
+    const int64_t b = l.chunk0 + i;
     const int ti = tensor_of(l, (uint32_t)b);
+    if (b >> 32) host_check::fail("a chunk number past 32 bits");
     if (ti < 0 || ti >= l.count || l.first[ti] > b) host_check::fail("a chunk without a tensor");
     else if ((b - l.first[ti]) * chunk >= l.t[ti].n) host_check::fail("a chunk behind the end of its tensor");
   }
@@ -575,20 +687,20 @@ int check_numel(const char* who, int64_t count, const int64_t* numel) {
   for (int64_t i = 0; i < count; ++i) {
     if (numel[i] < 0) return fail(MI_ERR_BAD_ARG, "%s: tensor %lld has a negative size", who, (long long)i);
     if (numel[i] > MAX_NUMEL)
-      return fail(MI_ERR_UNSUPPORTED_SHAPE, "%s: tensor %lld has %lld elements, at most 2^35 are supported", who, (long long)i, (long long)numel[i]);
+      return fail(MI_ERR_UNSUPPORTED_SHAPE, "%s: tensor %lld has %lld elements, at most 2^40 are supported", who, (long long)i, (long long)numel[i]);
   }
   return MI_OK;
 }
 
 template <class PT, class GT, class LT>
-int adam_launch(bool bits8, const AdamArgs& a, int64_t chunks, hipStream_t stream) {
+int adam_launch(bool bits8, const AdamArgs<LT>& a, int64_t chunks, hipStream_t stream) {
   const dim3 grid((unsigned)chunks), block(NT);
   if (bits8) hipLaunchKernelGGL((adamw8_kernel<PT, GT, LT>), grid, block, 0, stream, a);
   else hipLaunchKernelGGL((adamw_kernel<PT, GT, LT>), grid, block, 0, stream, a);
   return launched("mi_adamw_update");
 }
 template <class PT, class LT>
-int adam_launch_grad(int grad_dtype, bool bits8, const AdamArgs& a, int64_t chunks, hipStream_t stream) {
+int adam_launch_grad(int grad_dtype, bool bits8, const AdamArgs<LT>& a, int64_t chunks, hipStream_t stream) {
   if (grad_dtype == MI_DTYPE_F32) return adam_launch<PT, float, LT>(bits8, a, chunks, stream);
   if constexpr (!__is_same(PT, _Float16) && !__is_same(LT, _Float16))
     if (grad_dtype == MI_DTYPE_BF16) return adam_launch<PT, __bf16, LT>(bits8, a, chunks, stream);
@@ -631,8 +743,7 @@ int adam_impl(int64_t count, void* const* param, const void* const* grad, void* 
         if (!step_dev[i] || reinterpret_cast<uintptr_t>(step_dev[i]) % 4) return fail(MI_ERR_BAD_ARG, "%s: step %lld is null or not aligned", who, (long long)i);
     if (spans_conflict(spans)) return fail(MI_ERR_BAD_ARG, "%s: a tensor that is written overlaps another one of the call", who);
   }
-  AdamArgs a = {};
-  AdamScalars& s = a.s;
+  AdamScalars s = {};
   s.b1 = (float)beta1;
   s.omb1 = (float)(1.0 - beta1);
   s.b2 = (float)beta2;
@@ -649,31 +760,46 @@ int adam_impl(int64_t count, void* const* param, const void* const* grad, void* 
   s.grad_scale = grad_scale;
   decay_terms(decay_method, weight_decay, lr, &s.keep, &s.l2);
   if (!step_dev) bias_terms(s.ln_b1, s.ln_b2, step, lr, &s.step_size, &s.inv_sqrt_bc2);
-  const int64_t chunk = bits8 ? ADAM8_CHUNK : ADAM_CHUNK;
-  return for_each_list(
-      count, numel, chunk, a.list,
-      [&](int64_t i) {
-        return AdamTensor{param[i], grad[i], exp_avg[i], exp_avg_sq[i], model_param ? model_param[i] : nullptr, step_dev ? step_dev[i] : nullptr, numel[i]};
-      },
-      [&](const AdamList& l, int64_t chunks) -> int {
-        MI_OTHER_LAUNCH();
-        MI_WALK(l, chunks, chunk);
-        for (int i = 0; i < l.count; ++i) {
-          [[maybe_unused]] const AdamTensor& t = l.t[i];
-          [[maybe_unused]] const int64_t bytes8 = (int64_t)mi_moment_8bit_bytes(t.n);
-          MI_FOOTPRINT("weights", t.p, pb, 1, t.n, 1, t.n, t.n);
-          MI_FOOTPRINT("gradient", t.g, gb, 1, t.n, 1, t.n, t.n);
-          MI_FOOTPRINT("first moment", t.m, bits8 ? 1 : 4, 1, 0, 1, bits8 ? bytes8 : t.n, bits8 ? bytes8 : t.n);
-          MI_FOOTPRINT("second moment", t.v, bits8 ? 1 : 4, 1, 0, 1, bits8 ? bytes8 : t.n, bits8 ? bytes8 : t.n);
-          MI_FOOTPRINT("16-bit copy", t.low, 2, 1, 0, 1, t.n, t.n);
-        }
-        if (model_param)
-          return model_dtype == MI_DTYPE_BF16 ? adam_launch_grad<float, __bf16>(grad_dtype, bits8, a, chunks, stream)
-                                              : adam_launch_grad<float, _Float16>(grad_dtype, bits8, a, chunks, stream);
-        if (param_dtype == MI_DTYPE_F32) return adam_launch_grad<float, None>(grad_dtype, bits8, a, chunks, stream);
-        if (param_dtype == MI_DTYPE_BF16) return adam_launch_grad<__bf16, None>(grad_dtype, bits8, a, chunks, stream);
-        return adam_launch_grad<_Float16, None>(grad_dtype, bits8, a, chunks, stream);
-      });
+  const int64_t chunk = !bits8 ? ADAM_CHUNK : pb == 2 && gb == 2 ? Adam8Shape<__bf16, __bf16>::CHUNK : Adam8Shape<float, float>::CHUNK;
+  const auto entry = [&](int64_t i) { return AdamTensor{param[i], grad[i], exp_avg[i], exp_avg_sq[i], step_dev ? step_dev[i] : nullptr, numel[i]}; };
+  const auto state_footprints = [&](const auto& l, int64_t chunks) {
+    MI_OTHER_LAUNCH();
+    MI_WALK(l, chunks, chunk);
+    for (int i = 0; i < l.count; ++i) {
+      [[maybe_unused]] const AdamTensor& t = l.t[i];
+      [[maybe_unused]] const int64_t moment = bits8 ? (int64_t)mi_moment_8bit_bytes(t.n) : t.n;
+      MI_FOOTPRINT("weights", t.p, pb, 1, 0, 1, t.n, t.n);
+      MI_FOOTPRINT("gradient", t.g, gb, 1, 0, 1, t.n, t.n);
+      MI_FOOTPRINT("first moment", t.m, bits8 ? 1 : 4, 1, 0, 1, moment, moment);
+      MI_FOOTPRINT("second moment", t.v, bits8 ? 1 : 4, 1, 0, 1, moment, moment);
+    }
+  };
+  if (model_param) {
+    const auto run = [&](auto* a, auto launch) {
+      a->s = s;
+      return for_each_list(
+          count, numel, chunk, a->list, [&](int64_t i) { return AdamTensorCopy{entry(i), model_param[i]}; },
+          [&](const auto& l, int64_t chunks) -> int {
+            state_footprints(l, chunks);
+            for (int i = 0; i < l.count; ++i) MI_FOOTPRINT("16-bit copy", l.t[i].low, 2, 1, 0, 1, l.t[i].n, l.t[i].n);
+            return launch(*a, chunks);
+          });
+    };
+    if (model_dtype == MI_DTYPE_BF16) {
+      AdamArgs<__bf16> a;
+      return run(&a, [&](const auto& x, int64_t chunks) { return adam_launch_grad<float, __bf16>(grad_dtype, bits8, x, chunks, stream); });
+    }
+    AdamArgs<_Float16> a;
+    return run(&a, [&](const auto& x, int64_t chunks) { return adam_launch_grad<float, _Float16>(grad_dtype, bits8, x, chunks, stream); });
+  }
+  AdamArgs<None> a;
+  a.s = s;
+  return for_each_list(count, numel, chunk, a.list, entry, [&](const auto& l, int64_t chunks) -> int {
+    state_footprints(l, chunks);
+    if (param_dtype == MI_DTYPE_F32) return adam_launch_grad<float, None>(grad_dtype, bits8, a, chunks, stream);
+    if (param_dtype == MI_DTYPE_BF16) return adam_launch_grad<__bf16, None>(grad_dtype, bits8, a, chunks, stream);
+    return adam_launch_grad<_Float16, None>(grad_dtype, bits8, a, chunks, stream);
+  });
 }
 
 // Runs of equal data types are served by one launch each (as far as the argument block goes).
@@ -705,20 +831,20 @@ int check_list(const char* who, int64_t count, const void* const* x, const int64
   return MI_OK;
 }
 
-int norm_impl(int64_t count, const void* const* x, const int64_t* numel, const int* dtype, double max_norm, double* partials, size_t partials_len,
-              float* out, hipStream_t stream) {
-  const char* who = "mi_global_norm";
+// Partial sums of squares of a list.
+int sumsq_impl(const char* who, int64_t count, const void* const* x, const int64_t* numel, const int* dtype, double max_norm, double* partials,
+               size_t partials_len, float* out, int64_t* total, hipStream_t stream) {
   if (int rc = check_list(who, count, x, numel, dtype)) return rc;
   if (!out) return fail(MI_ERR_BAD_ARG, "%s: no output", who);
   if (!(max_norm >= 0.0)) return fail(MI_ERR_BAD_ARG, "%s: max_norm must not be negative", who);
-  const int64_t total = norm_chunks(count, numel);
-  if (total > 0 && (!partials || partials_len < (size_t)total))
-    return fail(MI_ERR_WORKSPACE, "%s: %lld partial sums are needed", who, (long long)total);
-  MI_FOOTPRINT("partial sums", partials, 8, 1, 0, 1, total, total);
+  *total = norm_chunks(count, numel);
+  if (*total > 0 && (!partials || partials_len < (size_t)*total))
+    return fail(MI_ERR_WORKSPACE, "%s: %lld partial sums are needed", who, (long long)*total);
+  MI_FOOTPRINT("partial sums", partials, 8, 1, 0, 1, *total, *total);
   MI_FOOTPRINT("norm and factor", out, 4, 1, 0, 1, 2, 2);
   int64_t done = 0;
   ReadList l;
-  const int rc = for_each_type(count, dtype, [&](int64_t at, int64_t len, int dt) {
+  return for_each_type(count, dtype, [&](int64_t at, int64_t len, int dt) {
     return for_each_list(
         len, numel + at, NORM_CHUNK, l, [&](int64_t i) { return ReadTensor{x[at + i], numel[at + i]}; },
         [&](const ReadList& list, int64_t chunks) -> int {
@@ -733,38 +859,72 @@ int norm_impl(int64_t count, const void* const* x, const int64_t* numel, const i
           return launched(who);
         });
   });
-  if (rc != MI_OK) return rc;
+}
+
+int finish_impl(const char* who, const double* partials, int64_t total, double max_norm, float* out, hipStream_t stream) {
   MI_OTHER_LAUNCH();
-  hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(1024), 0, stream, partials, total, (float)max_norm, out);
+  if (total <= FEW_PARTIALS) hipLaunchKernelGGL(norm_finish_kernel<NT>, dim3(1), dim3(NT), 0, stream, partials, total, (float)max_norm, out);
+  else hipLaunchKernelGGL(norm_finish_kernel<1024>, dim3(1), dim3(1024), 0, stream, partials, total, (float)max_norm, out);
   return launched(who);
 }
 
-int scale_impl(int64_t count, void* const* x, const int64_t* numel, const int* dtype, const float* factor, hipStream_t stream) {
-  const char* who = "mi_scale_tensors";
-  if (int rc = check_list(who, count, const_cast<const void* const*>(x), numel, dtype)) return rc;
-  if (!factor) return fail(MI_ERR_BAD_ARG, "%s: no factor", who);
+int overlap_impl(const char* who, int64_t count, const void* const* x, const int64_t* numel, const int* dtype) {
   std::vector<Span> spans;
   spans.reserve((size_t)count);
   for (int64_t i = 0; i < count; ++i) {
     const uintptr_t lo = reinterpret_cast<uintptr_t>(x[i]);
     if (numel[i] > 0) spans.push_back({lo, lo + (size_t)numel[i] * element_bytes(dtype[i]), true});
   }
-  if (spans_conflict(spans)) return fail(MI_ERR_BAD_ARG, "%s: two of the tensors overlap", who);
+  return spans_conflict(spans) ? fail(MI_ERR_BAD_ARG, "%s: two of the tensors overlap", who) : MI_OK;
+}
+
+template <bool FINISH>
+int scale_launches(const char* who, int64_t count, void* const* x, const int64_t* numel, const int* dtype, const ScaleFactor& sf, hipStream_t stream) {
   ReadList l;
   return for_each_type(count, dtype, [&](int64_t at, int64_t len, int dt) {
+    const int64_t chunk = dt == MI_DTYPE_F32 ? ScaleShape<float>::CHUNK : ScaleShape<__bf16>::CHUNK;
     return for_each_list(
-        len, numel + at, SCALE_CHUNK, l, [&](int64_t i) { return ReadTensor{x[at + i], numel[at + i]}; },
+        len, numel + at, chunk, l, [&](int64_t i) { return ReadTensor{x[at + i], numel[at + i]}; },
         [&](const ReadList& list, int64_t chunks) -> int {
           MI_OTHER_LAUNCH();
-          MI_WALK(list, chunks, SCALE_CHUNK);
+          MI_WALK(list, chunks, chunk);
           for (int i = 0; i < list.count; ++i) MI_FOOTPRINT("tensor", list.t[i].x, element_bytes(dt), 1, 0, 1, list.t[i].n, list.t[i].n);
           const dim3 grid((unsigned)chunks), block(NT);
-          if (dt == MI_DTYPE_F32) hipLaunchKernelGGL(scale_list_kernel<float>, grid, block, 0, stream, list, factor);
-          else if (dt == MI_DTYPE_BF16) hipLaunchKernelGGL(scale_list_kernel<__bf16>, grid, block, 0, stream, list, factor);
-          else hipLaunchKernelGGL(scale_list_kernel<_Float16>, grid, block, 0, stream, list, factor);
+          if (dt == MI_DTYPE_F32) hipLaunchKernelGGL((scale_list_kernel<float, FINISH>), grid, block, 0, stream, list, sf);
+          else if (dt == MI_DTYPE_BF16) hipLaunchKernelGGL((scale_list_kernel<__bf16, FINISH>), grid, block, 0, stream, list, sf);
+          else hipLaunchKernelGGL((scale_list_kernel<_Float16, FINISH>), grid, block, 0, stream, list, sf);
           return launched(who);
         });
   });
+}
+
+int norm_impl(int64_t count, const void* const* x, const int64_t* numel, const int* dtype, double max_norm, double* partials, size_t partials_len,
+              float* out, hipStream_t stream) {
+  const char* who = "mi_global_norm";
+  int64_t total = 0;
+  if (int rc = sumsq_impl(who, count, x, numel, dtype, max_norm, partials, partials_len, out, &total, stream)) return rc;
+  return finish_impl(who, partials, total, max_norm, out, stream);
+}
+
+int scale_impl(int64_t count, void* const* x, const int64_t* numel, const int* dtype, const float* factor, hipStream_t stream) {
+  const char* who = "mi_scale_tensors";
+  if (int rc = check_list(who, count, x, numel, dtype)) return rc;
+  if (!factor) return fail(MI_ERR_BAD_ARG, "%s: no factor", who);
+  if (int rc = overlap_impl(who, count, x, numel, dtype)) return rc;
+  return scale_launches<false>(who, count, x, numel, dtype, ScaleFactor{factor, nullptr, 0, 0.0f, nullptr}, stream);
+}
+
+int clip_impl(int64_t count, void* const* x, const int64_t* numel, const int* dtype, double max_norm, double* partials, size_t partials_len, float* out,
+              hipStream_t stream) {
+  const char* who = "mi_clip_by_global_norm";
+  if (int rc = check_list(who, count, x, numel, dtype)) return rc;
+  if (int rc = overlap_impl(who, count, x, numel, dtype)) return rc;
+  int64_t total = 0;
+  if (int rc = sumsq_impl(who, count, x, numel, dtype, max_norm, partials, partials_len, out, &total, stream)) return rc;
+  if (total > 0 && total <= FEW_PARTIALS)
+    return scale_launches<true>(who, count, x, numel, dtype, ScaleFactor{nullptr, partials, total, (float)max_norm, out}, stream);
+  if (int rc = finish_impl(who, partials, total, max_norm, out, stream)) return rc;
+  return scale_launches<false>(who, count, x, numel, dtype, ScaleFactor{out + 1, nullptr, 0, 0.0f, nullptr}, stream);
 }
 
 template <class T>
@@ -789,12 +949,13 @@ int move_impl(bool pack, int64_t count, const void* const* src, void* const* dst
     if (int rc = add_spans(who, "destination", spans, count, const_cast<const void* const*>(dst), numel, element_bytes(dtype), pack, true)) return rc;
     if (spans_conflict(spans)) return fail(MI_ERR_BAD_ARG, "%s: a tensor that is written overlaps another one of the call", who);
   }
+  const int64_t chunk = dtype == MI_DTYPE_F32 ? MoveShape<float>::CHUNK : MoveShape<__bf16>::CHUNK;
   MoveList l;
   return for_each_list(
-      count, numel, MOVE_CHUNK, l, [&](int64_t i) { return MoveTensor{src[i], dst[i], numel[i]}; },
+      count, numel, chunk, l, [&](int64_t i) { return MoveTensor{src[i], dst[i], numel[i]}; },
       [&](const MoveList& list, int64_t chunks) -> int {
         MI_OTHER_LAUNCH();
-        MI_WALK(list, chunks, MOVE_CHUNK);
+        MI_WALK(list, chunks, chunk);
         for (int i = 0; i < list.count; ++i) {
           [[maybe_unused]] const MoveTensor& t = list.t[i];
           [[maybe_unused]] const int64_t bytes8 = (int64_t)mi_moment_8bit_bytes(t.n);
@@ -842,6 +1003,12 @@ size_t mi_global_norm_partials_len(int64_t count, const int64_t* numel) {
 int mi_global_norm(int64_t count, const void* const* x, const int64_t* numel, const int* dtype, double max_norm, double* partials,
                    size_t partials_len, float* out, void* stream) {
   return mi::norm_impl(count, x, numel, dtype, max_norm, partials, partials_len, out, static_cast<hipStream_t>(stream));
+}
+
+int mi_clip_by_global_norm(int64_t count, void* const* x, const int64_t* numel, const int* dtype, double max_norm, double* partials,
+                           size_t partials_len, float* out, void* stream) {
+  return mi::guarded("mi_clip_by_global_norm",
+                     [&] { return mi::clip_impl(count, x, numel, dtype, max_norm, partials, partials_len, out, static_cast<hipStream_t>(stream)); });
 }
 
 int mi_scale_tensors(int64_t count, void* const* x, const int64_t* numel, const int* dtype, const float* factor, void* stream) {

@@ -9,8 +9,11 @@ working accelerated path.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
+from types import ModuleType
 from typing import Optional
 
 import torch
@@ -62,6 +65,7 @@ EXPORTS = (
     ),
     ("mi_global_norm_partials_len", _sz, (_i64, _vp)),
     ("mi_global_norm", _int, (_i64, _vp, _vp, _vp, _f64, _vp, _sz, _vp, _vp)),
+    ("mi_clip_by_global_norm", _int, (_i64, _vp, _vp, _vp, _f64, _vp, _sz, _vp, _vp)),
     ("mi_scale_tensors", _int, (_i64, _vp, _vp, _vp, _vp, _vp)),
     ("mi_moment_8bit_bytes", _sz, (_i64,)),
     ("mi_moments_8bit_pack", _int, (_i64, _vp, _vp, _vp, _int, _int, _vp)),
@@ -109,6 +113,29 @@ def lib() -> ctypes.CDLL:
     if _lib is None:
         raise RuntimeError(f"HIP extension unavailable: {_load_error}")
     return _lib
+
+
+LISTS_PATH = os.path.join(_CSRC_DIR, "_mi_lists.so")
+_lists: Optional[ModuleType] = None
+
+
+def lists() -> ModuleType:
+    """The module that reads lists of tensors for the multi-tensor entries (``csrc/tensor_lists.cpp``); raises
+    ``RuntimeError`` when it is missing (no fallback)."""
+    global _lists
+    if _lists is None:
+        lib()
+        if not os.path.exists(LISTS_PATH):
+            raise RuntimeError(f"HIP extension unavailable: {LISTS_PATH} not found; build it with `make -C {_CSRC_DIR}`")
+        try:
+            loader = importlib.machinery.ExtensionFileLoader("_mi_lists", LISTS_PATH)
+            spec = importlib.util.spec_from_file_location("_mi_lists", LISTS_PATH, loader=loader)
+            module = importlib.util.module_from_spec(spec)
+            loader.exec_module(module)
+        except ImportError as exc:  # built for another Python or torch
+            raise RuntimeError(f"HIP extension unavailable: cannot load {LISTS_PATH}: {exc}") from exc
+        _lists = module
+    return _lists
 
 
 _gfx950: dict[int, bool] = {}

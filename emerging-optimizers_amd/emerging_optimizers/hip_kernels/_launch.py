@@ -2,10 +2,7 @@
 
 from __future__ import annotations
 
-import array
-import contextlib
 import ctypes
-from typing import ContextManager, Sequence
 
 import torch
 
@@ -63,24 +60,8 @@ def syrk_launch(
     _hip.check(rc)
 
 
-# ---------------------------------------------------------------------------------------------
-# lists of tensors
-# ---------------------------------------------------------------------------------------------
-#: MI_DTYPE_* codes of the library
-DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
-
-def on_device(index: int) -> ContextManager:
-    """Makes GPU ``index`` the current one, at no cost where it already is."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index)
-
-
-def pointers(tensors: Sequence[torch.Tensor]) -> array.array:
-    return array.array("q", map(torch.Tensor.data_ptr, tensors))
-
-
-def address(a: array.array | None) -> int | None:
-    return None if a is None else a.buffer_info()[0]
+#: Data types of the multi-tensor operators
+LIST_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def is_dense(t: torch.Tensor) -> bool:
@@ -93,35 +74,3 @@ def is_dense(t: torch.Tensor) -> bool:
             return False
         want *= size
     return True
-
-
-def list_device(who: str, *lists: Sequence[torch.Tensor]) -> int:
-    """The one GPU all tensors of the lists are on."""
-    found = set()
-    for tensors in lists:
-        found.update(map(torch.Tensor.get_device, tensors))
-    if -1 in found:
-        raise RuntimeError(f"{who} runs on the GPU only; got a tensor on the CPU")
-    if len(found) != 1:
-        raise ValueError(f"{who}: all tensors of a call must be on one GPU, got {sorted(found)}")
-    return found.pop()
-
-
-def list_dtype(who: str, what: str, tensors: Sequence[torch.Tensor], allowed: Sequence[torch.dtype] = tuple(DTYPE_CODES)) -> torch.dtype:
-    """The one data type of the tensors of a list."""
-    found = {t.dtype for t in tensors}
-    if len(found) != 1 or not found <= set(allowed):
-        names = ", ".join(sorted(str(d) for d in found))
-        raise TypeError(f"{who}: {what} must have one data type out of {', '.join(str(d) for d in allowed)}, got {names}")
-    return found.pop()
-
-
-def check_like(who: str, what: str, tensors: Sequence[torch.Tensor], like: Sequence[torch.Tensor]) -> None:
-    """``tensors`` have the shapes and the memory order of ``like``, whose elements fill their memory."""
-    if len(tensors) != len(like):
-        raise ValueError(f"{who}: {len(tensors)} {what} for {len(like)} params")
-    for i, (t, p) in enumerate(zip(tensors, like)):
-        if t.shape != p.shape:
-            raise ValueError(f"{who}: {what}[{i}] has shape {tuple(t.shape)}, its param {tuple(p.shape)}")
-        if not (t.is_contiguous() and p.is_contiguous()) and (t.stride() != p.stride() or not is_dense(p)):
-            raise ValueError(f"{who}: {what}[{i}] must fill its memory in the order of its param, got strides {t.stride()} and {p.stride()}")

@@ -7,7 +7,6 @@ from typing import Literal, Optional, Sequence, Union
 import torch
 
 from .. import _hip
-from . import _launch
 
 
 __all__ = ["fused_adamw_update", "fused_adamw_update_8bit", "moment_8bit_bytes", "pack_moments_8bit", "unpack_moments_8bit"]
@@ -23,81 +22,11 @@ def moment_8bit_bytes(numel: int) -> int:
     return -(-numel // 64) * 68
 
 
-def _check_packed(who: str, what: str, packed: Sequence[torch.Tensor], like: Sequence[torch.Tensor]) -> None:
-    if len(packed) != len(like):
-        raise ValueError(f"{who}: {len(packed)} {what} for {len(like)} tensors")
-    for i, (t, p) in enumerate(zip(packed, like)):
-        if t.dtype != torch.uint8:
-            raise TypeError(f"{who}: {what}[{i}] must be uint8, got {t.dtype}")
-        if t.numel() != moment_8bit_bytes(p.numel()) or not t.is_contiguous():
-            raise ValueError(f"{who}: {what}[{i}] must be {moment_8bit_bytes(p.numel())} contiguous bytes, got {tuple(t.shape)}")
-
-
-def _device_scalar(who: str, what: str, t: torch.Tensor, device: int) -> torch.Tensor:
-    if t.dtype != torch.float32 or t.numel() != 1 or t.get_device() != device:
-        raise ValueError(f"{who}: {what} must be one float32 value on the GPU of the params, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t
-
-
-def _adamw(
-    who: str,
-    bits: int,
-    params: Sequence[torch.Tensor],
-    grads: Sequence[torch.Tensor],
-    exp_avgs: Sequence[torch.Tensor],
-    exp_avg_sqs: Sequence[torch.Tensor],
-    step: Union[float, Sequence[torch.Tensor]],
-    lr: Union[float, torch.Tensor],
-    beta1: float,
-    beta2: float,
-    eps: float,
-    weight_decay: float,
-    weight_decay_method: str,
-    grad_scale: Optional[torch.Tensor],
-    model_params: Optional[Sequence[torch.Tensor]],
-) -> None:
-    method = _DECAY_METHODS.get(weight_decay_method)
-    if method is None:
-        raise ValueError(f"Invalid weight decay method: {weight_decay_method}")
-    if len(params) == 0 and len(grads) == len(exp_avgs) == len(exp_avg_sqs) == len(model_params or ()) == 0:
-        return
-    p_type = _launch.list_dtype(who, "params", params)
-    g_type = _launch.list_dtype(who, "grads", grads)
-    _launch.check_like(who, "grads", grads, params)
-    if bits == 32:
-        for what, moments in (("exp_avgs", exp_avgs), ("exp_avg_sqs", exp_avg_sqs)):
-            _launch.list_dtype(who, what, moments, (torch.float32,))
-            _launch.check_like(who, what, moments, params)
-    else:
-        _check_packed(who, "exp_avgs", exp_avgs, params)
-        _check_packed(who, "exp_avg_sqs", exp_avg_sqs, params)
-    low_type = torch.bfloat16
-    if model_params is not None:
-        if p_type != torch.float32:
-            raise TypeError(f"{who}: model_params go with float32 params, got {p_type}")
-        low_type = _launch.list_dtype(who, "model_params", model_params, (torch.bfloat16, torch.float16))
-        _launch.check_like(who, "model_params", model_params, params)
-    device = _launch.list_device(who, params, grads, exp_avgs, exp_avg_sqs, model_params or ())
-    steps = None
-    if not isinstance(step, (int, float)):
-        if len(step) != len(params):
-            raise ValueError(f"{who}: {len(step)} steps for {len(params)} params")
-        steps = _launch.pointers([_device_scalar(who, "step", t, device) for t in step])
-    lr_ptr = None
-    if isinstance(lr, torch.Tensor):
-        lr_ptr, lr = _device_scalar(who, "lr", lr, device).data_ptr(), 0.0
-    scale_ptr = None if grad_scale is None else _device_scalar(who, "grad_scale", grad_scale, device).data_ptr()
-    lists = [_launch.pointers(t) for t in (params, grads, exp_avgs, exp_avg_sqs)]
-    low = None if model_params is None else _launch.pointers(model_params)
-    numels = _launch.array.array("q", map(torch.Tensor.numel, params))
-    with _launch.on_device(device):
-        rc = _hip.lib().mi_adamw_update(
-            len(params), *map(_launch.address, lists), _launch.address(low), _launch.address(steps), _launch.address(numels),
-            _launch.DTYPE_CODES[p_type], _launch.DTYPE_CODES[g_type], _launch.DTYPE_CODES[low_type], bits,
-            1.0 if steps is not None else float(step), float(lr), lr_ptr, float(beta1), float(beta2), float(eps),
-            float(weight_decay), method, scale_ptr, torch.cuda.current_stream().cuda_stream,
-        )  # fmt: skip
-    _hip.check(rc)
+def _decay_code(method: str) -> int:
+    code = _DECAY_METHODS.get(method)
+    if code is None:
+        raise ValueError(f"Invalid weight decay method: {method}")
+    return code
 
 
 def fused_adamw_update(
@@ -139,10 +68,11 @@ def fused_adamw_update(
     written may share memory with another one.  Any size from 0 on, any alignment.  The work is enqueued on the current
     stream of the tensors' GPU; nothing waits.
     """
-    _adamw(
-        "fused_adamw_update", 32, params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps, weight_decay,
-        weight_decay_method, grad_scale, model_params,
+    rc = _hip.lists().adamw_update(
+        "fused_adamw_update", 32, params, grads, exp_avgs, exp_avg_sqs, model_params, step, lr, beta1, beta2, eps, weight_decay,
+        _decay_code(weight_decay_method), grad_scale,
     )  # fmt: skip
+    _hip.check(rc)
 
 
 def fused_adamw_update_8bit(
@@ -165,33 +95,18 @@ def fused_adamw_update_8bit(
     of :func:`moment_8bit_bytes` bytes each, 16-byte aligned (zeros stand for zero moments; see
     :func:`pack_moments_8bit`).  The update uses the new moments before they are rounded to 8 bits.
     """
-    _adamw(
-        "fused_adamw_update_8bit", 8, params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps, weight_decay,
-        weight_decay_method, grad_scale, model_params,
+    rc = _hip.lists().adamw_update(
+        "fused_adamw_update_8bit", 8, params, grads, exp_avgs, exp_avg_sqs, model_params, step, lr, beta1, beta2, eps, weight_decay,
+        _decay_code(weight_decay_method), grad_scale,
     )  # fmt: skip
+    _hip.check(rc)
 
 
 def _move(who: str, pack: bool, values: Sequence[torch.Tensor], packed: Sequence[torch.Tensor], which: MomentT) -> None:
     second = _MOMENTS.get(which)
     if second is None:
         raise ValueError(f'{who}: which must be "exp_avg" or "exp_avg_sq", got {which!r}')
-    _check_packed(who, "packed", packed, values)
-    if len(values) == 0:
-        return
-    dtype = _launch.list_dtype(who, "moments", values)
-    if not all(map(_launch.is_dense, values)):
-        raise ValueError(f"{who}: moments must fill their memory")
-    device = _launch.list_device(who, values, packed)
-    v, q = _launch.pointers(values), _launch.pointers(packed)
-    numels = _launch.array.array("q", map(torch.Tensor.numel, values))
-    src, dst = (v, q) if pack else (q, v)
-    lib = _hip.lib()
-    with _launch.on_device(device):
-        rc = (lib.mi_moments_8bit_pack if pack else lib.mi_moments_8bit_unpack)(
-            len(values), _launch.address(src), _launch.address(dst), _launch.address(numels), _launch.DTYPE_CODES[dtype], second,
-            torch.cuda.current_stream().cuda_stream,
-        )  # fmt: skip
-    _hip.check(rc)
+    _hip.check(_hip.lists().move_moments(who, pack, values, packed, second))
 
 
 def pack_moments_8bit(moments: Sequence[torch.Tensor], packed: Sequence[torch.Tensor], *, which: MomentT) -> None:

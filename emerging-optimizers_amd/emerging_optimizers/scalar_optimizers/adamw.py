@@ -16,7 +16,7 @@ import torch
 from torch.optim.optimizer import Optimizer, ParamsT
 
 from emerging_optimizers import hip_kernels
-from emerging_optimizers.hip_kernels._launch import DTYPE_CODES, is_dense
+from emerging_optimizers.hip_kernels._launch import LIST_DTYPES, is_dense
 from emerging_optimizers.mixin import WeightDecayMixin, WeightDecayT
 
 
@@ -123,7 +123,7 @@ class AdamW(WeightDecayMixin, Optimizer):
                 continue
             if not is_dense(p):
                 raise ValueError("AdamW needs parameters that fill their memory")
-            if self.moment_bits == 8 and p.dtype not in DTYPE_CODES:
+            if self.moment_bits == 8 and p.dtype not in LIST_DTYPES:
                 raise ValueError(f"8-bit moments need float32, bfloat16 or float16 parameters, got {p.dtype}")
             state["step"] = self._first_step(p)
             state["exp_avg"] = self._moment(p)
@@ -168,7 +168,7 @@ class AdamW(WeightDecayMixin, Optimizer):
 
     @staticmethod
     def _kernels_take(p: torch.Tensor, held: torch.Tensor) -> bool:
-        if not (hip_kernels.on_kernel_device(p) and p.dtype in DTYPE_CODES and p.grad.dtype in DTYPE_CODES):
+        if not (hip_kernels.on_kernel_device(p) and p.dtype in LIST_DTYPES and p.grad.dtype in LIST_DTYPES):
             return False
         hip_kernels.require_library()
         half = {torch.bfloat16, torch.float16}

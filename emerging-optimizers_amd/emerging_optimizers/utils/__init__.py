@@ -8,7 +8,7 @@ from typing import Iterable, Iterator, Literal, Union
 import torch
 
 from emerging_optimizers import hip_kernels
-from emerging_optimizers.hip_kernels._launch import DTYPE_CODES, is_dense
+from emerging_optimizers.hip_kernels._launch import LIST_DTYPES, is_dense
 
 
 __all__ = ["clip_grad_norm_", "fp32_matmul_precision", "FP32MatmulPrecT"]
@@ -50,7 +50,7 @@ def clip_grad_norm_(
     if not grads:
         return torch.tensor(0.0)
     kernels = len({g.device for g in grads}) == 1 and all(
-        hip_kernels.on_kernel_device(g) and g.dtype in DTYPE_CODES and is_dense(g) for g in grads
+        hip_kernels.on_kernel_device(g) and g.dtype in LIST_DTYPES and is_dense(g) for g in grads
     )
     if kernels and not error_if_nonfinite:
         return hip_kernels.clip_grads_by_global_norm(grads, max_norm=max_norm)

@@ -220,8 +220,8 @@ int mi_muon_update_bf16(float* param, const float* grad, float* momentum, int64_
  *
  * A list is `count` device pointers in a HOST array, with the element counts in another; the arrays are read during the
  * call only.  Tensors are contiguous, need the alignment of their elements only (8-bit moments: 16 bytes) and may have
- * any size from 0 to 2^35 elements.  No tensor that a call writes may overlap another tensor of the call.  One launch
- * serves up to 60 tensors (192 for the norm and the scaling, 128 for the conversions); nothing is allocated, copied
+ * any size from 0 to 2^40 elements.  No tensor that a call writes may overlap another tensor of the call.  One launch
+ * serves up to 76 tensors (66 with 16-bit copies, 192 for norm and scaling, 128 for the conversions); nothing is allocated, copied
  * or waited for, so calls may be captured into a HIP graph (with a step count on the device where it has to advance).
  */
 #define MI_DTYPE_F32 0
@@ -261,6 +261,13 @@ int mi_adamw_update(int64_t count, void* const* param, const void* const* grad, 
 size_t mi_global_norm_partials_len(int64_t count, const int64_t* numel);
 int mi_global_norm(int64_t count, const void* const* x, const int64_t* numel, const int* dtype, double max_norm,
                    double* partials, size_t partials_len, float* out, void* stream);
+
+/*
+ * mi_global_norm, and x <- out[1] * x for every tensor of the list (nothing is written where out[1] is 1).  Tensors
+ * must not overlap.  Two launches for lists whose partial sums are few, three and more for others.
+ */
+int mi_clip_by_global_norm(int64_t count, void* const* x, const int64_t* numel, const int* dtype, double max_norm,
+                           double* partials, size_t partials_len, float* out, void* stream);
 
 /* x <- *factor * x for every tensor of the list (factor: float32 on the device; exactly 1 leaves everything alone). */
 int mi_scale_tensors(int64_t count, void* const* x, const int64_t* numel, const int* dtype, const float* factor,

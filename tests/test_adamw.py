@@ -45,7 +45,7 @@ def adamw_rc(p=(1 << 20,), g=(2 << 20,), m=(3 << 20,), v=(4 << 20,), low=None, n
     [
         (dict(count=-1), _hip.MI_ERR_BAD_ARG, "bad tensor count"),
         (dict(n=(-5,)), _hip.MI_ERR_BAD_ARG, "negative size"),
-        (dict(n=((1 << 35) + 1,)), _hip.MI_ERR_UNSUPPORTED_SHAPE, "2\\^35"),
+        (dict(n=((1 << 40) + 1,)), _hip.MI_ERR_UNSUPPORTED_SHAPE, "2\\^40"),
         (dict(p=(0,)), _hip.MI_ERR_BAD_ARG, "param 0 is null"),
         (dict(g=(0,)), _hip.MI_ERR_BAD_ARG, "grad 0 is null"),
         (dict(m=None), _hip.MI_ERR_BAD_ARG, "no list of exp_avg"),
@@ -104,10 +104,12 @@ def test_norm_scale_and_conversion_entries_refuse():
         ((2, None, at(n), at(f32), 1.0, 4096, need, 8192), _hip.MI_ERR_BAD_ARG, "no list"),
         ((2, at(longs(1 << 20, 2)), at(n), at(f32), 1.0, 4096, need, 8192), _hip.MI_ERR_BAD_ARG, "tensor 1 is null or not aligned"),
     ):
-        assert lib.mi_global_norm(*args, None) == code and text in _hip.last_error()
+        for fn in (lib.mi_global_norm, lib.mi_clip_by_global_norm):
+            assert fn(*args, None) == code and text in _hip.last_error()
     assert lib.mi_scale_tensors(2, at(x), at(n), at(f32), None, None) == _hip.MI_ERR_BAD_ARG and "no factor" in _hip.last_error()
     same = longs(1 << 20, (1 << 20) + 3996)
     assert lib.mi_scale_tensors(2, at(same), at(n), at(f32), 64, None) == _hip.MI_ERR_BAD_ARG and "overlap" in _hip.last_error()
+    assert lib.mi_clip_by_global_norm(2, at(same), at(n), at(f32), 1.0, 4096, need, 8192, None) == _hip.MI_ERR_BAD_ARG and "overlap" in _hip.last_error()
     for fn in (lib.mi_moments_8bit_pack, lib.mi_moments_8bit_unpack):
         assert fn(2, at(x), at(longs(3 << 20, 4 << 20)), at(n), 7, 0, None) == _hip.MI_ERR_BAD_ARG and "data type" in _hip.last_error()
         assert fn(2, at(x), at(longs(3 << 20, 4 << 20)), at(n), 0, 2, None) == _hip.MI_ERR_BAD_ARG and "moment" in _hip.last_error()

@@ -228,6 +228,25 @@ def test_zero_gradients_and_moments_keep_weights_and_nan_stays_in_its_place(gpu,
         assert m[70].isnan() and m[150].isinf() and v[150].isinf() and not m[~bad].any()
 
 
+def test_the_same_memory_twice_and_half_aligned_moments_are_refused(gpu):
+    """Refused on the host before any launch; nothing changes."""
+    p, g, m, v = (torch.ones(100, device=gpu) for _ in range(4))
+    for lists in (([p, p], [g, g], [m, m.clone()], [v, v.clone()]), ([p], [g], [m], [m]), ([p], [p], [m], [v]), ([p[:60], p[50:]], [g[:60], g[50:]], [m[:60], m[50:]], [v[:60], v[50:]])):
+        with pytest.raises(ValueError, match="overlaps"):
+            k.fused_adamw_update(*lists, step=1, **HYPER)
+    with pytest.raises(ValueError, match="overlap"):
+        k.clip_grads_by_global_norm([g, g], max_norm=1e-3)
+    packed = torch.zeros(2 * 136 + 8, dtype=torch.uint8, device=gpu)
+    with pytest.raises(ValueError, match="aligned to 16"):
+        k.fused_adamw_update_8bit([p], [g], [packed[8:144]], [packed[144:280]], step=1, **HYPER)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        k.fused_adamw_update([p], [g], [m], [v.cpu()], step=1, **HYPER)
+    with pytest.raises(ValueError, match="grad_scale must be one float32"):
+        k.fused_adamw_update([p], [g], [m], [v], step=1, grad_scale=torch.ones(2, device=gpu), **HYPER)
+    for t in (p, g, m, v):
+        assert torch.all(t == 1)
+
+
 def test_extreme_magnitudes_keep_within_float32(gpu):
     """Gradients whose squares underflow leave the update to eps; weights of any size survive."""
     for scale in (1e-30, 1e-20, 1e-10, 1e3, 1e15):
@@ -357,6 +376,51 @@ def test_norm_is_the_same_every_time(gpu):
     grads = values(gen, [1 << 20, 12345, 7], 1.0)
     first = k.global_grad_norm(grads)
     assert all(torch.equal(first, k.global_grad_norm(grads)) for _ in range(5))
+
+
+def test_a_tensor_of_more_than_two_to_the_33_values(gpu):
+    """Offsets past 32 bits, more chunks than one launch takes: slices of a huge bfloat16 tensor that is zero elsewhere,
+    against the same slices as tensors of their own."""
+    n = (1 << 33) + 4099
+    if torch.cuda.mem_get_info()[0] < 90 << 30:
+        pytest.skip("needs 90 GiB of free GPU memory")
+    gen = torch.Generator().manual_seed(17)
+    p, g, out = (torch.zeros(n, dtype=BF16, device=gpu) for _ in range(3))
+    packed = [torch.zeros(k.moment_8bit_bytes(n), dtype=torch.uint8, device=gpu) for _ in range(2)]
+    places = [slice(a, a + 4096) for a in (0, (1 << 31) - 2048, (1 << 32) - 2048, (1 << 33) - 2048)] + [slice(n - 1987, n)]
+    small_p, small_g = [], []
+    for place in places:
+        p[place] = (torch.randn(place.stop - place.start, generator=gen) * 0.02).to(BF16).to(gpu)
+        g[place] = torch.randn(place.stop - place.start, generator=gen).to(BF16).to(gpu)
+        small_p.append(p[place].clone())
+        small_g.append(g[place].clone())
+    norm, factor = k.global_grad_norm([g], max_norm=0.5)
+    small_norm, small_factor = k.global_grad_norm(small_g, max_norm=0.5)
+    assert abs(float(norm) - float(small_norm)) <= 2 * O.U * float(norm)  # (another order of the float64 sums)
+    small = [[torch.zeros(k.moment_8bit_bytes(x.numel()), dtype=torch.uint8, device=gpu) for x in small_p] for _ in range(2)]
+    for step in (1, 2):
+        k.fused_adamw_update_8bit([p], [g], [packed[0]], [packed[1]], step=step, grad_scale=factor, **HYPER)
+        k.fused_adamw_update_8bit(small_p, small_g, *small, step=step, grad_scale=factor, **HYPER)
+    for place, want in zip(places, small_p):
+        assert torch.equal(p[place], want)
+        assert not p[place.stop : place.stop + 64].any() and not p[max(place.start - 64, 0) : place.start].any()
+    for mine, theirs, which in zip(packed, small, ("exp_avg", "exp_avg_sq")):
+        k.unpack_moments_8bit([mine], [out], which=which)
+        for place, q in zip(places, theirs):
+            want = torch.empty(place.stop - place.start, dtype=BF16, device=gpu)
+            k.unpack_moments_8bit([q], [want], which=which)
+            assert torch.equal(out[place], want) and want.any()
+            assert not out[place.stop : place.stop + 64].any()
+        k.pack_moments_8bit([out], [mine], which=which)
+        for place in places:
+            again = [torch.empty(k.moment_8bit_bytes(place.stop - place.start), dtype=torch.uint8, device=gpu)]
+            k.pack_moments_8bit([out[place]], again, which=which)
+            codes = again[0][: place.stop - place.start]
+            assert torch.equal(mine[place], codes) and codes.any()
+    norm = k.clip_grads_by_global_norm([g], max_norm=0.5)
+    k.scale_tensors(small_g, factor)
+    for place, want in zip(places, small_g):
+        assert torch.equal(g[place], want) and want.any()
 
 
 # ---------------------------------------------------------------------------------------------
