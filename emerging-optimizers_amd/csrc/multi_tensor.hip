@@ -19,7 +19,7 @@
 namespace mi {
 namespace {
 
-constexpr int NT = 256;  // threads of a workgroup
+constexpr int NT = 256;  // threads of a workgroup where nothing else is said
 constexpr int BLOCK8 = 64;  // values that share a scale in the 8-bit form of a moment
 // A launch's workgroup count stays below 2^24 (2^32 threads) with room to spare; a tensor of more chunks takes several
 // launches.  Chunks of one tensor are numbered in 32 bits.
@@ -182,8 +182,8 @@ __device__ __forceinline__ void adam_value(float& p, float g, float& m, float& v
 
 // 32-bit moments.  Each value is read and written once: 28 bytes a value with float32 weights and gradients, about 25
 // operations, so the memory bounds it.
-constexpr int ADAM_V = 4, ADAM_U = 1;
-constexpr int ADAM_CHUNK = NT * ADAM_V * ADAM_U;
+constexpr int ADAM_V = 4;
+constexpr int ADAM_CHUNK = NT * ADAM_V;
 
 template <class PT, class GT, class LT>
 __global__ __launch_bounds__(NT) void adamw_kernel(AdamArgs<LT> a) {
@@ -199,41 +199,39 @@ __global__ __launch_bounds__(NT) void adamw_kernel(AdamArgs<LT> a) {
   float* __restrict__ v = static_cast<float*>(t.v) + base;
   const int64_t left = t.n - base;
   const AdamCoef c = adam_coefficients(a.s, t.step);
-  for (int u = 0; u < ADAM_U; ++u) {
-    const int e = (u * NT + threadIdx.x) * V;
-    if (e >= left) return;
-    const int k = left - e < V ? (int)(left - e) : V;
-    F pp, gg, mm, vv;
-    if (k == V) {
-      gg = load<V>(g + e);
-      pp = load<V>(p + e);
-      mm = load<V>(m + e);
-      vv = load<V>(v + e);
-    } else {
-      gg = load_part<V>(g + e, k);
-      pp = load_part<V>(p + e, k);
-      mm = load_part<V>(m + e, k);
-      vv = load_part<V>(v + e, k);
-    }
+  const int e = threadIdx.x * V;
+  if (e >= left) return;
+  const int k = left - e < V ? (int)(left - e) : V;
+  F pp, gg, mm, vv;
+  if (k == V) {
+    gg = load<V>(g + e);
+    pp = load<V>(p + e);
+    mm = load<V>(m + e);
+    vv = load<V>(v + e);
+  } else {
+    gg = load_part<V>(g + e, k);
+    pp = load_part<V>(p + e, k);
+    mm = load_part<V>(m + e, k);
+    vv = load_part<V>(v + e, k);
+  }
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float pi = pp[i], mi = mm[i], vi = vv[i];
-      adam_value<false>(pi, gg[i], mi, vi, c);
-      pp[i] = pi;
-      mm[i] = mi;
-      vv[i] = vi;
-    }
-    if (k == V) {
-      store<V>(p + e, pp);
-      store<V>(m + e, mm);
-      store<V>(v + e, vv);
-      if constexpr (!__is_same(LT, None)) store<V>(static_cast<LT*>(t.low) + base + e, pp);
-    } else {
-      store_part<V>(p + e, pp, k);
-      store_part<V>(m + e, mm, k);
-      store_part<V>(v + e, vv, k);
-      if constexpr (!__is_same(LT, None)) store_part<V>(static_cast<LT*>(t.low) + base + e, pp, k);
-    }
+  for (int i = 0; i < V; ++i) {
+    float pi = pp[i], mi = mm[i], vi = vv[i];
+    adam_value<false>(pi, gg[i], mi, vi, c);
+    pp[i] = pi;
+    mm[i] = mi;
+    vv[i] = vi;
+  }
+  if (k == V) {
+    store<V>(p + e, pp);
+    store<V>(m + e, mm);
+    store<V>(v + e, vv);
+    if constexpr (!__is_same(LT, None)) store<V>(static_cast<LT*>(t.low) + base + e, pp);
+  } else {
+    store_part<V>(p + e, pp, k);
+    store_part<V>(m + e, mm, k);
+    store_part<V>(v + e, vv, k);
+    if constexpr (!__is_same(LT, None)) store_part<V>(static_cast<LT*>(t.low) + base + e, pp, k);
   }
 }
 
@@ -332,8 +330,7 @@ __device__ __forceinline__ void store_codes(uint8_t* p, Codes<V> codes) {
 
 template <class PT, class GT>
 struct Adam8Shape {
-  static constexpr int V = sizeof(PT) == 2 && sizeof(GT) == 2 ? 8 : 4, U = 1;
-  static constexpr int CHUNK = NT * V * U;
+  static constexpr int V = sizeof(PT) == 2 && sizeof(GT) == 2 ? 8 : 4, CHUNK = NT * V;
 };
 
 template <class PT, class GT, class LT>
@@ -354,60 +351,58 @@ __global__ __launch_bounds__(NT) void adamw8_kernel(AdamArgs<LT> a) {
   float* __restrict__ vs = reinterpret_cast<float*>(static_cast<uint8_t*>(t.v) + nb * BLOCK8) + base / BLOCK8;
   const int64_t left = t.n - base;
   const AdamCoef c = adam_coefficients(a.s, t.step);
-  for (int u = 0; u < S::U; ++u) {
-    const int e = (u * NT + threadIdx.x) * V;
-    const int b = e / BLOCK8;
-    if ((int64_t)b * BLOCK8 >= left) return;  // all lanes of the block together
-    const int k = left - e >= V ? V : left - e > 0 ? (int)(left - e) : 0;
-    F pp, gg;
-    if (k == V) {
-      pp = load<V>(p + e);
-      gg = load<V>(g + e);
-    } else {
-      pp = load_part<V>(p + e, k);
-      gg = load_part<V>(g + e, k);
-    }
-    F mm = decode<V, true>(load_codes<V>(mc + e), ms[b]), vv = decode<V, false>(load_codes<V>(vc + e), vs[b]);
+  const int e = threadIdx.x * V;
+  const int b = e / BLOCK8;
+  if ((int64_t)b * BLOCK8 >= left) return;  // all lanes of the block together
+  const int k = left - e >= V ? V : left - e > 0 ? (int)(left - e) : 0;
+  F pp, gg;
+  if (k == V) {
+    pp = load<V>(p + e);
+    gg = load<V>(g + e);
+  } else {
+    pp = load_part<V>(p + e, k);
+    gg = load_part<V>(g + e, k);
+  }
+  F mm = decode<V, true>(load_codes<V>(mc + e), ms[b]), vv = decode<V, false>(load_codes<V>(vc + e), vs[b]);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float pi = pp[i], mi = mm[i], vi = vv[i];
-      adam_value<true>(pi, gg[i], mi, vi, c);
-      pp[i] = pi;
-      mm[i] = mi;
-      vv[i] = vi;
-    }
-    if (k < V) {  // places behind the last value hold 0
+  for (int i = 0; i < V; ++i) {
+    float pi = pp[i], mi = mm[i], vi = vv[i];
+    adam_value<true>(pi, gg[i], mi, vi, c);
+    pp[i] = pi;
+    mm[i] = mi;
+    vv[i] = vi;
+  }
+  if (k < V) {  // places behind the last value hold 0
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (i >= k) mm[i] = vv[i] = 0.0f;
-    }
-    const float sm = block_scale<V>(mm), sv = block_scale<V>(vv);
-    store_codes<V>(mc + e, encode<V, true>(mm, sm));
-    store_codes<V>(vc + e, encode<V, false>(vv, sv));
-    if (e % BLOCK8 == 0) {
-      ms[b] = sm;
-      vs[b] = sv;
-    }
-    if (k == V) {
-      store<V>(p + e, pp);
-      if constexpr (!__is_same(LT, None)) store<V>(static_cast<LT*>(t.low) + base + e, pp);
-    } else {
-      store_part<V>(p + e, pp, k);
-      if constexpr (!__is_same(LT, None)) store_part<V>(static_cast<LT*>(t.low) + base + e, pp, k);
-    }
+    for (int i = 0; i < V; ++i)
+      if (i >= k) mm[i] = vv[i] = 0.0f;
+  }
+  const float sm = block_scale<V>(mm), sv = block_scale<V>(vv);
+  store_codes<V>(mc + e, encode<V, true>(mm, sm));
+  store_codes<V>(vc + e, encode<V, false>(vv, sv));
+  if (e % BLOCK8 == 0) {
+    ms[b] = sm;
+    vs[b] = sv;
+  }
+  if (k == V) {
+    store<V>(p + e, pp);
+    if constexpr (!__is_same(LT, None)) store<V>(static_cast<LT*>(t.low) + base + e, pp);
+  } else {
+    store_part<V>(p + e, pp, k);
+    if constexpr (!__is_same(LT, None)) store_part<V>(static_cast<LT*>(t.low) + base + e, pp, k);
   }
 }
 
 // Conversions between a list of tensors and their 8-bit forms.
-template <class T>
+template <class T, bool PACK>
 struct MoveShape {
-  static constexpr int V = sizeof(T) == 2 ? 8 : 4, U = 2;
-  static constexpr int CHUNK = NT * V * U;
+  static constexpr int V = sizeof(T) == 2 ? 8 : 4, U = sizeof(T) == 4 && !PACK ? 4 : 2, THREADS = 128;
+  static constexpr int CHUNK = THREADS * V * U;
 };
 
 template <class T, bool SIGNED>
-__global__ __launch_bounds__(NT) void pack8_kernel(MoveList l) {
-  typedef MoveShape<T> S;
+__global__ __launch_bounds__((MoveShape<T, true>::THREADS)) void pack8_kernel(MoveList l) {
+  typedef MoveShape<T, true> S;
   constexpr int V = S::V;
   const uint32_t chunk = l.chunk0 + blockIdx.x;
   const int ti = tensor_of(l, chunk);
@@ -419,7 +414,7 @@ __global__ __launch_bounds__(NT) void pack8_kernel(MoveList l) {
   const int64_t left = t.n - base;
 #pragma unroll
   for (int u = 0; u < S::U; ++u) {
-    const int e = (u * NT + threadIdx.x) * V;
+    const int e = (u * S::THREADS + threadIdx.x) * V;
     const int b = e / BLOCK8;
     if ((int64_t)b * BLOCK8 >= left) return;  // all lanes of the block together
     const int k = left - e >= V ? V : left - e > 0 ? (int)(left - e) : 0;
@@ -431,8 +426,8 @@ __global__ __launch_bounds__(NT) void pack8_kernel(MoveList l) {
 }
 
 template <class T, bool SIGNED>
-__global__ __launch_bounds__(NT) void unpack8_kernel(MoveList l) {
-  typedef MoveShape<T> S;
+__global__ __launch_bounds__((MoveShape<T, false>::THREADS)) void unpack8_kernel(MoveList l) {
+  typedef MoveShape<T, false> S;
   constexpr int V = S::V;
   const uint32_t chunk = l.chunk0 + blockIdx.x;
   const int ti = tensor_of(l, chunk);
@@ -444,7 +439,7 @@ __global__ __launch_bounds__(NT) void unpack8_kernel(MoveList l) {
   const int64_t left = t.n - base;
 #pragma unroll
   for (int u = 0; u < S::U; ++u) {
-    const int e = (u * NT + threadIdx.x) * V;
+    const int e = (u * S::THREADS + threadIdx.x) * V;
     if (e >= left) return;
     const Floats<V> xx = decode<V, SIGNED>(load_codes<V>(codes + e), scales[e / BLOCK8]);
     if (left - e >= V) store<V>(x + e, xx);
@@ -651,24 +646,44 @@ void walk(const L& l, int64_t chunks, int64_t chunk) {
 int element_bytes(int dtype) { return dtype == MI_DTYPE_F32 ? 4 : 2; }
 bool known_dtype(int dtype) { return dtype == MI_DTYPE_F32 || dtype == MI_DTYPE_BF16 || dtype == MI_DTYPE_F16; }
 
-// Memory of a call: no written range may meet any other.
+// Memory of a call: no written range may meet any other.  The ranges come role by role (weights, gradients, ...); the
+// addresses of a role mostly ascend already, so the roles are merged and only one that does not ascend is sorted.
 struct Span {
   uintptr_t lo, hi;
-  bool written;
 };
-bool spans_conflict(std::vector<Span>& spans) {
-  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
-  uintptr_t end_any = 0, end_written = 0;
-  for (const Span& s : spans) {
-    if (s.lo < (s.written ? end_any : end_written)) return true;
-    end_any = std::max(end_any, s.hi);
-    if (s.written) end_written = std::max(end_written, s.hi);
+struct Spans {
+  static constexpr int MAX_ROLES = 5;
+  std::vector<Span> all;
+  size_t end[MAX_ROLES] = {};
+  bool written[MAX_ROLES] = {};
+  int roles = 0;
+
+  void close_role(bool is_written) {
+    const size_t begin = roles ? end[roles - 1] : 0;
+    const auto before = [](const Span& a, const Span& b) { return a.lo < b.lo; };
+    if (!std::is_sorted(all.begin() + begin, all.end(), before)) std::sort(all.begin() + begin, all.end(), before);
+    written[roles] = is_written;
+    end[roles++] = all.size();
   }
-  return false;
-}
+  bool conflict() const {
+    size_t head[MAX_ROLES];
+    for (int r = 0; r < roles; ++r) head[r] = r ? end[r - 1] : 0;
+    uintptr_t end_any = 0, end_written = 0;
+    for (;;) {
+      int r = -1;
+      for (int i = 0; i < roles; ++i)
+        if (head[i] < end[i] && (r < 0 || all[head[i]].lo < all[head[r]].lo)) r = i;
+      if (r < 0) return false;
+      const Span& s = all[head[r]++];
+      if (s.lo < (written[r] ? end_any : end_written)) return true;
+      end_any = std::max(end_any, s.hi);
+      if (written[r]) end_written = std::max(end_written, s.hi);
+    }
+  }
+};
 
 // Checks one list argument and adds its ranges.
-int add_spans(const char* who, const char* what, std::vector<Span>& spans, int64_t count, const void* const* ptrs, const int64_t* numel,
+int add_spans(const char* who, const char* what, Spans& spans, int64_t count, const void* const* ptrs, const int64_t* numel,
               int bytes, bool packed, bool written) {
   if (!ptrs && count > 0) return fail(MI_ERR_BAD_ARG, "%s: no list of %s", who, what);
   const uintptr_t align = packed ? 16 : (uintptr_t)bytes;
@@ -677,8 +692,9 @@ int add_spans(const char* who, const char* what, std::vector<Span>& spans, int64
     const uintptr_t lo = reinterpret_cast<uintptr_t>(ptrs[i]);
     if (!lo) return fail(MI_ERR_BAD_ARG, "%s: %s %lld is null", who, what, (long long)i);
     if (lo % align) return fail(MI_ERR_BAD_ARG, "%s: %s %lld is not aligned to %d bytes", who, what, (long long)i, (int)align);
-    spans.push_back({lo, lo + (packed ? mi_moment_8bit_bytes(numel[i]) : (size_t)numel[i] * bytes), written});
+    spans.all.push_back({lo, lo + (packed ? mi_moment_8bit_bytes(numel[i]) : (size_t)numel[i] * bytes)});
   }
+  spans.close_role(written);
   return MI_OK;
 }
 
@@ -694,9 +710,9 @@ int check_numel(const char* who, int64_t count, const int64_t* numel) {
 
 template <class PT, class GT, class LT>
 int adam_launch(bool bits8, const AdamArgs<LT>& a, int64_t chunks, hipStream_t stream) {
-  const dim3 grid((unsigned)chunks), block(NT);
-  if (bits8) hipLaunchKernelGGL((adamw8_kernel<PT, GT, LT>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((adamw_kernel<PT, GT, LT>), grid, block, 0, stream, a);
+  const dim3 grid((unsigned)chunks);
+  if (bits8) hipLaunchKernelGGL((adamw8_kernel<PT, GT, LT>), grid, dim3(NT), 0, stream, a);
+  else hipLaunchKernelGGL((adamw_kernel<PT, GT, LT>), grid, dim3(NT), 0, stream, a);
   return launched("mi_adamw_update");
 }
 template <class PT, class LT>
@@ -730,8 +746,8 @@ int adam_impl(int64_t count, void* const* param, const void* const* grad, void* 
   const bool bits8 = moment_bits == 8;
   const int pb = element_bytes(param_dtype), gb = element_bytes(grad_dtype);
   {
-    std::vector<Span> spans;
-    spans.reserve((size_t)count * (model_param ? 5 : 4));
+    Spans spans;
+    spans.all.reserve((size_t)count * (model_param ? 5 : 4));
     if (int rc = add_spans(who, "param", spans, count, const_cast<const void* const*>(param), numel, pb, false, true)) return rc;
     if (int rc = add_spans(who, "grad", spans, count, grad, numel, gb, false, false)) return rc;
     if (int rc = add_spans(who, "exp_avg", spans, count, const_cast<const void* const*>(exp_avg), numel, 4, bits8, true)) return rc;
@@ -741,7 +757,7 @@ int adam_impl(int64_t count, void* const* param, const void* const* grad, void* 
     if (step_dev)
       for (int64_t i = 0; i < count; ++i)
         if (!step_dev[i] || reinterpret_cast<uintptr_t>(step_dev[i]) % 4) return fail(MI_ERR_BAD_ARG, "%s: step %lld is null or not aligned", who, (long long)i);
-    if (spans_conflict(spans)) return fail(MI_ERR_BAD_ARG, "%s: a tensor that is written overlaps another one of the call", who);
+    if (spans.conflict()) return fail(MI_ERR_BAD_ARG, "%s: a tensor that is written overlaps another one of the call", who);
   }
   AdamScalars s = {};
   s.b1 = (float)beta1;
@@ -869,13 +885,14 @@ int finish_impl(const char* who, const double* partials, int64_t total, double m
 }
 
 int overlap_impl(const char* who, int64_t count, const void* const* x, const int64_t* numel, const int* dtype) {
-  std::vector<Span> spans;
-  spans.reserve((size_t)count);
+  Spans spans;
+  spans.all.reserve((size_t)count);
   for (int64_t i = 0; i < count; ++i) {
     const uintptr_t lo = reinterpret_cast<uintptr_t>(x[i]);
-    if (numel[i] > 0) spans.push_back({lo, lo + (size_t)numel[i] * element_bytes(dtype[i]), true});
+    if (numel[i] > 0) spans.all.push_back({lo, lo + (size_t)numel[i] * element_bytes(dtype[i])});
   }
-  return spans_conflict(spans) ? fail(MI_ERR_BAD_ARG, "%s: two of the tensors overlap", who) : MI_OK;
+  spans.close_role(true);
+  return spans.conflict() ? fail(MI_ERR_BAD_ARG, "%s: two of the tensors overlap", who) : MI_OK;
 }
 
 template <bool FINISH>
@@ -929,11 +946,11 @@ int clip_impl(int64_t count, void* const* x, const int64_t* numel, const int* dt
 
 template <class T>
 int move_launch(bool pack, bool second, const MoveList& l, int64_t chunks, hipStream_t stream, const char* who) {
-  const dim3 grid((unsigned)chunks), block(NT);
-  if (pack && !second) hipLaunchKernelGGL((pack8_kernel<T, true>), grid, block, 0, stream, l);
-  else if (pack) hipLaunchKernelGGL((pack8_kernel<T, false>), grid, block, 0, stream, l);
-  else if (!second) hipLaunchKernelGGL((unpack8_kernel<T, true>), grid, block, 0, stream, l);
-  else hipLaunchKernelGGL((unpack8_kernel<T, false>), grid, block, 0, stream, l);
+  const dim3 grid((unsigned)chunks), packing(MoveShape<T, true>::THREADS), unpacking(MoveShape<T, false>::THREADS);
+  if (pack && !second) hipLaunchKernelGGL((pack8_kernel<T, true>), grid, packing, 0, stream, l);
+  else if (pack) hipLaunchKernelGGL((pack8_kernel<T, false>), grid, packing, 0, stream, l);
+  else if (!second) hipLaunchKernelGGL((unpack8_kernel<T, true>), grid, unpacking, 0, stream, l);
+  else hipLaunchKernelGGL((unpack8_kernel<T, false>), grid, unpacking, 0, stream, l);
   return launched(who);
 }
 
@@ -943,13 +960,14 @@ int move_impl(bool pack, int64_t count, const void* const* src, void* const* dst
   if (!known_dtype(dtype)) return fail(MI_ERR_BAD_ARG, "%s: unknown data type", who);
   if (second != 0 && second != 1) return fail(MI_ERR_BAD_ARG, "%s: the moment is 0 (first) or 1 (second), got %d", who, second);
   {
-    std::vector<Span> spans;
-    spans.reserve((size_t)count * 2);
+    Spans spans;
+    spans.all.reserve((size_t)count * 2);
     if (int rc = add_spans(who, "source", spans, count, src, numel, element_bytes(dtype), !pack, false)) return rc;
     if (int rc = add_spans(who, "destination", spans, count, const_cast<const void* const*>(dst), numel, element_bytes(dtype), pack, true)) return rc;
-    if (spans_conflict(spans)) return fail(MI_ERR_BAD_ARG, "%s: a tensor that is written overlaps another one of the call", who);
+    if (spans.conflict()) return fail(MI_ERR_BAD_ARG, "%s: a tensor that is written overlaps another one of the call", who);
   }
-  const int64_t chunk = dtype == MI_DTYPE_F32 ? MoveShape<float>::CHUNK : MoveShape<__bf16>::CHUNK;
+  const int64_t chunk = dtype == MI_DTYPE_F32 ? (pack ? MoveShape<float, true>::CHUNK : MoveShape<float, false>::CHUNK) : MoveShape<__bf16, true>::CHUNK;
+  static_assert(MoveShape<__bf16, true>::CHUNK == MoveShape<__bf16, false>::CHUNK, "one chunk for both directions");
   MoveList l;
   return for_each_list(
       count, numel, chunk, l, [&](int64_t i) { return MoveTensor{src[i], dst[i], numel[i]}; },

@@ -147,44 +147,50 @@ class AdamW(WeightDecayMixin, Optimizer):
             self._init_group(group)
             batches: dict = {}
             for p in group["params"]:
-                if p.grad is None:
+                grad = p.grad
+                if grad is None:
                     continue
-                if p.grad.is_sparse:
+                if grad.is_sparse:
                     raise RuntimeError("AdamW does not support sparse gradients")
                 state = self.state[p]
                 if not self.capturable:
                     state["step"] += 1
-                held = state.get("master", p)
-                if self._kernels_take(p, held):
-                    key = (p.device, p.dtype, p.grad.dtype, held is p, None if self.capturable else state["step"])
-                    batches.setdefault(key, []).append(p)
-                else:
+                key = (p.get_device(), p.dtype, grad.dtype, "master" in state, None if self.capturable else state["step"])
+                batch = batches.get(key)
+                if batch is None:
+                    batch = batches[key] = (self._kernels_take(p, grad), [], [], [])
+                batch[1].append(p)
+                batch[2].append(grad)
+                batch[3].append(state)
+            for kernels, params, grads, states in batches.values():
+                if kernels:
+                    self._update_batch(params, grads, states, group, grad_scale)
+                    continue
+                for p, state in zip(params, states):
                     if self.capturable:
                         state["step"] += 1
                     self._update_torch(p, group, grad_scale)
-            for members in batches.values():
-                self._update_batch(members, group, grad_scale)
         return None
 
     @staticmethod
-    def _kernels_take(p: torch.Tensor, held: torch.Tensor) -> bool:
-        if not (hip_kernels.on_kernel_device(p) and p.dtype in LIST_DTYPES and p.grad.dtype in LIST_DTYPES):
+    def _kernels_take(p: torch.Tensor, grad: torch.Tensor) -> bool:
+        """Whether the kernels serve the device and the types of ``p`` and its gradient."""
+        if not (hip_kernels.on_kernel_device(p) and p.dtype in LIST_DTYPES and grad.dtype in LIST_DTYPES):
             return False
         hip_kernels.require_library()
-        half = {torch.bfloat16, torch.float16}
-        return p.dtype not in half or p.grad.dtype not in half or p.dtype == p.grad.dtype
+        return torch.float32 in (p.dtype, grad.dtype) or p.dtype == grad.dtype
 
-    def _update_batch(self, members: list, group: dict, grad_scale: Optional[torch.Tensor]) -> None:
+    def _update_batch(self, params: list, grads: list, states: list, group: dict, grad_scale: Optional[torch.Tensor]) -> None:
         """One call for parameters of one device, type and step."""
-        states = [self.state[p] for p in members]
-        grads = [p.grad if p.grad.stride() == p.stride() else torch.empty_like(p, dtype=p.grad.dtype).copy_(p.grad) for p in members]
+        if not all(map(torch.Tensor.is_contiguous, params)) or not all(map(torch.Tensor.is_contiguous, grads)):
+            grads = [g if g.stride() == p.stride() else torch.empty_like(p, dtype=g.dtype).copy_(g) for p, g in zip(params, grads)]
         step: Any = states[0]["step"]
         if self.capturable:
             step = [s["step"] for s in states]
             torch._foreach_add_(step, 1)
         masters = "master" in states[0]
         (hip_kernels.fused_adamw_update if self.moment_bits == 32 else hip_kernels.fused_adamw_update_8bit)(
-            [s["master"] for s in states] if masters else [p.detach() for p in members],
+            [s["master"] for s in states] if masters else params,
             grads,
             [s["exp_avg"] for s in states],
             [s["exp_avg_sq"] for s in states],
@@ -196,7 +202,7 @@ class AdamW(WeightDecayMixin, Optimizer):
             weight_decay=group["weight_decay"],
             weight_decay_method=self.weight_decay_method,
             grad_scale=grad_scale,
-            model_params=[p.detach() for p in members] if masters else None,
+            model_params=params if masters else None,
         )
 
     def _update_torch(self, p: torch.Tensor, group: dict, grad_scale: Optional[torch.Tensor]) -> None:
