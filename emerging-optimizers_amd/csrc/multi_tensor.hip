@@ -10,7 +10,7 @@
 #include <stdint.h>
 
 #include <algorithm>
-#include <new>
+#include <exception>
 #include <vector>
 
 #include "../../include/mi_ns.h"
@@ -991,8 +991,8 @@ template <class Body>
 int guarded(const char* who, Body body) {
   try {
     return body();
-  } catch (const std::bad_alloc&) {
-    return fail(MI_ERR_BAD_ARG, "%s: out of host memory", who);
+  } catch (const std::exception& e) {
+    return fail(MI_ERR_BAD_ARG, "%s: %s", who, e.what());
   }
 }
 

@@ -136,6 +136,12 @@ struct List {
     for (size_t i = 0; i < t.size(); ++i) p[i] = t[i]->data_ptr();
     return p;
   }
+  // The call writes these tensors: autograd's version counters move as after an in-place operation, so a backward pass
+  // over a graph that saved one of them is refused.
+  void written() const {
+    for (const at::Tensor* x : t)
+      if (!x->is_inference()) x->unsafeGetTensorImpl()->bump_version();
+  }
   std::vector<int64_t> numels() const {
     std::vector<int64_t> n(t.size());
     for (size_t i = 0; i < t.size(); ++i) n[i] = t[i]->numel();
@@ -239,7 +245,7 @@ PyObject* adamw_update(PyObject*, PyObject* args) {
     const c10::Device device = one_gpu(who, {&params, &grads, &ms, &vs, has_low ? &low : nullptr});
     std::vector<const float*> steps;
     double step = 1.0, lr = 0.0;
-    if (PyFloat_Check(step_) || PyLong_Check(step_)) {
+    if (PyNumber_Check(step_) && !PySequence_Check(step_)) {
       step = number_of(who, "step", step_);
     } else {
       const List s(who, "step", step_);
@@ -255,9 +261,16 @@ PyObject* adamw_update(PyObject*, PyObject* args) {
     if (has_low) l = low.pointers();
     const std::vector<int64_t> n = params.numels();
     const c10::DeviceGuard guard(device);
-    return PyLong_FromLong(mi_adamw_update((int64_t)p.size(), p.data(), g.data(), m.data(), v.data(), has_low ? l.data() : nullptr,
-                                           steps.empty() ? nullptr : steps.data(), n.data(), p_type, g_type, low_type, bits, step, lr, lr_dev, beta1, beta2, eps, wd,
-                                           method, scale, current_stream(device)));
+    const int rc = mi_adamw_update((int64_t)p.size(), p.data(), g.data(), m.data(), v.data(), has_low ? l.data() : nullptr,
+                                   steps.empty() ? nullptr : steps.data(), n.data(), p_type, g_type, low_type, bits, step, lr, lr_dev, beta1, beta2, eps, wd, method,
+                                   scale, current_stream(device));
+    if (rc == MI_OK) {
+      params.written();
+      ms.written();
+      vs.written();
+      if (has_low) low.written();
+    }
+    return PyLong_FromLong(rc);
   });
 }
 
@@ -278,8 +291,10 @@ PyObject* move_moments(PyObject*, PyObject* args) {
     const std::vector<int64_t> n = values.numels();
     const c10::DeviceGuard guard(device);
     void* const stream = current_stream(device);
-    return PyLong_FromLong(pack ? mi_moments_8bit_pack((int64_t)x.size(), x.data(), q.data(), n.data(), type, second, stream)
-                                : mi_moments_8bit_unpack((int64_t)x.size(), q.data(), x.data(), n.data(), type, second, stream));
+    const int rc = pack ? mi_moments_8bit_pack((int64_t)x.size(), x.data(), q.data(), n.data(), type, second, stream)
+                        : mi_moments_8bit_unpack((int64_t)x.size(), q.data(), x.data(), n.data(), type, second, stream);
+    if (rc == MI_OK) (pack ? packed : values).written();
+    return PyLong_FromLong(rc);
   });
 }
 
@@ -311,6 +326,7 @@ PyObject* global_norm(PyObject*, PyObject* args) {
     double* const scratch = length ? static_cast<double*>(partials.data_ptr()) : nullptr;
     const int rc = scale ? mi_clip_by_global_norm(count, x.data(), n.data(), types.data(), max_norm, scratch, length, result, stream)
                          : mi_global_norm(count, x.data(), n.data(), types.data(), max_norm, scratch, length, result, stream);
+    if (rc == MI_OK && scale) tensors.written();
     return Py_BuildValue("(iNN)", rc, THPVariable_Wrap(out.select(0, 0)), THPVariable_Wrap(out.select(0, 1)));
   });
 }
@@ -330,7 +346,9 @@ PyObject* scale_tensors(PyObject*, PyObject* args) {
     const std::vector<void*> x = tensors.pointers();
     const std::vector<int64_t> n = tensors.numels();
     const c10::DeviceGuard guard(device);
-    return PyLong_FromLong(mi_scale_tensors(tensors.size(), x.data(), n.data(), types.data(), factor, current_stream(device)));
+    const int rc = mi_scale_tensors(tensors.size(), x.data(), n.data(), types.data(), factor, current_stream(device));
+    if (rc == MI_OK) tensors.written();
+    return PyLong_FromLong(rc);
   });
 }
 

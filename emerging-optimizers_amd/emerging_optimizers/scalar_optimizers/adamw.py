@@ -51,11 +51,6 @@ def _unpack_torch(packed: torch.Tensor, numel: int, which: str) -> torch.Tensor:
     return (k * k * scale)[:numel]
 
 
-def _memory_order(t: torch.Tensor) -> torch.Tensor:
-    """Flat view of a dense tensor in the order of its memory."""
-    return t.as_strided((t.numel(),), (1,))
-
-
 class AdamW(WeightDecayMixin, Optimizer):
     """Adam with decoupled weight decay (arXiv:1711.05101), one call for all parameters of a kind.
 
@@ -112,6 +107,15 @@ class AdamW(WeightDecayMixin, Optimizer):
     def _first_step(self, p: torch.Tensor) -> Any:
         return torch.zeros((), dtype=torch.float32, device=p.device) if self.capturable else 0
 
+    def _check_param(self, p: torch.Tensor) -> None:
+        if not is_dense(p):
+            raise ValueError("AdamW needs parameters that fill their memory")
+        if self.moment_bits == 8 and p.dtype not in LIST_DTYPES:
+            raise ValueError(f"8-bit moments need float32, bfloat16 or float16 parameters, got {p.dtype}")
+        if self.moment_bits == 8 and not p.is_contiguous():
+            # their bytes say nothing about an order of the dimensions, so a checkpoint could not be checked against it
+            raise ValueError("8-bit moments need contiguous parameters")
+
     @torch.no_grad()
     def _init_group(self, group: dict, skip_non_grad_params: bool = True) -> None:
         """Creates the state of every parameter of ``group`` that does not have one yet."""
@@ -121,10 +125,10 @@ class AdamW(WeightDecayMixin, Optimizer):
             state = self.state[p]
             if state:
                 continue
-            if not is_dense(p):
-                raise ValueError("AdamW needs parameters that fill their memory")
-            if self.moment_bits == 8 and p.dtype not in LIST_DTYPES:
-                raise ValueError(f"8-bit moments need float32, bfloat16 or float16 parameters, got {p.dtype}")
+            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+                # the zeros would be part of the graph and every replay would start from them
+                raise RuntimeError("AdamW needs a step before the one that is captured, to make its state")
+            self._check_param(p)
             state["step"] = self._first_step(p)
             state["exp_avg"] = self._moment(p)
             state["exp_avg_sq"] = self._moment(p)
@@ -215,7 +219,7 @@ class AdamW(WeightDecayMixin, Optimizer):
             grad.mul_(grad_scale)
         self._apply_weight_decay_inplace(w, grad, lr, group["weight_decay"])
         if self.moment_bits == 8:
-            m, v = (_unpack_torch(state[k], p.numel(), k).as_strided(w.shape, w.stride()) for k in ("exp_avg", "exp_avg_sq"))
+            m, v = (_unpack_torch(state[k], p.numel(), k).view(w.shape) for k in ("exp_avg", "exp_avg_sq"))
         else:
             m, v = state["exp_avg"], state["exp_avg_sq"]
         m.lerp_(grad, 1 - beta1)
@@ -225,7 +229,7 @@ class AdamW(WeightDecayMixin, Optimizer):
         w.sub_(lr / (1 - beta1**t) * (m / den))
         if self.moment_bits == 8:
             for k, x in (("exp_avg", m), ("exp_avg_sq", v)):
-                state[k].copy_(_pack_torch(_memory_order(x), k))
+                state[k].copy_(_pack_torch(x.reshape(-1), k))
         held.copy_(w)
         if held is not p:
             p.copy_(w)
@@ -241,34 +245,34 @@ class AdamW(WeightDecayMixin, Optimizer):
                 if index not in saved:
                     continue
                 state = self.state[p]
+                self._check_param(p)
                 # (the base class casts what it loads to the parameter's type)
                 state["exp_avg"], state["exp_avg_sq"] = (self._loaded_moment(saved[index][k], p, k) for k in ("exp_avg", "exp_avg_sq"))
                 step = float(saved[index]["step"])
                 state["step"] = self._first_step(p).fill_(step) if self.capturable else int(step)
                 if self.master_weights and p.dtype in (torch.bfloat16, torch.float16):
-                    state["master"] = saved[index].get("master", p.detach()).to(device=p.device, dtype=torch.float32, copy=True)
+                    state["master"] = torch.empty_like(p, dtype=torch.float32).copy_(saved[index].get("master", p.detach()))
                 else:
                     state.pop("master", None)
 
     def _loaded_moment(self, value: torch.Tensor, p: torch.Tensor, which: str) -> torch.Tensor:
+        """A moment of a checkpoint in the width and the memory order that this optimizer holds it in."""
         packed = value.dtype == torch.uint8 and value.dim() == 1
-        if packed and value.numel() != hip_kernels.moment_8bit_bytes(p.numel()):
-            raise ValueError(f"{which} of {value.numel()} bytes for a parameter of {p.numel()} values")
-        if packed and self.moment_bits == 8:
-            return value.to(p.device, copy=True)
-        new = self._moment(p)
+        if packed and value.numel() != hip_kernels.moment_8bit_bytes(p.numel()) or not packed and value.shape != p.shape:
+            raise ValueError(f"{which} of shape {tuple(value.shape)} for a parameter of shape {tuple(p.shape)}")
+        if packed == (self.moment_bits == 8):
+            return value.to(p.device, copy=True) if packed else self._moment(p).copy_(value)
         kernels = hip_kernels.on_kernel_device(p)
-        if not packed:
-            wide = torch.empty_like(p, dtype=torch.promote_types(p.dtype, torch.float32)).copy_(value)
-            if self.moment_bits == 32:
-                return wide
+        if packed:
+            value, wide = value.to(p.device), torch.empty(p.shape, device=p.device, dtype=torch.float32)
             if kernels:
-                hip_kernels.pack_moments_8bit([wide], [new], which=which)
-                return new
-            return new.copy_(_pack_torch(_memory_order(wide), which))
-        value = value.to(p.device)
-        if kernels and new.dtype == torch.float32:
-            hip_kernels.unpack_moments_8bit([value], [new], which=which)
+                hip_kernels.unpack_moments_8bit([value], [wide], which=which)
+            else:
+                wide.copy_(_unpack_torch(value, p.numel(), which).view(p.shape))
+            return self._moment(p).copy_(wide)
+        wide, new = value.to(p.device, torch.float32).contiguous(), self._moment(p)
+        if kernels:
+            hip_kernels.pack_moments_8bit([wide], [new], which=which)
         else:
-            _memory_order(new).copy_(_unpack_torch(value, p.numel(), which))
+            new.copy_(_pack_torch(wide.view(-1), which))
         return new

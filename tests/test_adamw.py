@@ -354,8 +354,37 @@ def test_checkpoints_between_widths_and_with_torch_on_the_cpu():
     narrow2 = AdamW([other], moment_bits=8)
     saved = narrow.state_dict()
     saved["state"][0].pop("master", None)
-    with pytest.raises(ValueError, match="bytes for a parameter"):
+    with pytest.raises(ValueError, match="for a parameter of shape"):
         narrow2.load_state_dict(saved)
+
+
+def test_checkpoints_of_transposed_parameters():
+    """Moments are held in the memory order of their parameter, whatever order the checkpoint's have; 8-bit ones say
+    nothing about an order and need contiguous parameters."""
+    gen = torch.Generator().manual_seed(5)
+    a = torch.nn.Parameter(torch.randn(6, 10, generator=gen))
+    b = torch.nn.Parameter(a.detach().t().contiguous().t())
+    assert not b.is_contiguous()
+    opts = [AdamW([p], lr=0.1) for p in (a, b)]
+    for turn in range(2):
+        g = torch.randn(6, 10, generator=gen)
+        for p, opt in zip((a, b), opts):
+            p.grad = g.clone()
+            opt.step()
+        assert torch.equal(a, b)
+        opts[1] = AdamW([b], lr=0.1)
+        opts[1].load_state_dict(opts[0].state_dict())
+        assert opts[1].state[b]["exp_avg"].stride() == b.stride()
+    with pytest.raises(ValueError, match="contiguous"):
+        AdamW([b], moment_bits=8).step()
+    with pytest.raises(ValueError, match="contiguous"):
+        AdamW([b], moment_bits=8).load_state_dict(opts[0].state_dict())
+    narrow = AdamW([a], lr=0.1, moment_bits=8)
+    narrow.load_state_dict(opts[0].state_dict())
+    opts[1].load_state_dict(narrow.state_dict())
+    want = O.decode(narrow.state[a]["exp_avg"].numpy(), 60, "exp_avg")[0].reshape(6, 10)
+    assert opts[1].state[b]["exp_avg"].stride() == b.stride()
+    O.assert_within(opts[1].state[b]["exp_avg"].numpy(), want, 8 * O.U * abs(want) + 1e-300, "read back")
 
 
 def test_clip_grad_norm_on_the_cpu():

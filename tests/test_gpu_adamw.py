@@ -497,6 +497,38 @@ def test_capture_needs_a_step_count_on_the_device(gpu):
             opt.step()
 
 
+def test_state_is_not_made_inside_a_capture(gpu):
+    p = torch.nn.Parameter(torch.ones(10, device=gpu))
+    p.grad = torch.ones_like(p)
+    opt = AdamW([p], capturable=True)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="before the one that is captured"):
+        with torch.cuda.graph(graph):
+            opt.step()
+    assert p not in opt.state or not opt.state[p]
+    opt.step()
+    assert float(opt.state[p]["step"]) == 1
+
+
+def test_autograd_notices_what_the_calls_write(gpu):
+    """Version counters move with every tensor that a call writes, so a graph that saved one of them refuses to go on."""
+    p = torch.nn.Parameter(torch.ones(10, device=gpu))
+    loss = (p * p).sum()
+    p.grad = torch.ones_like(p)
+    m, v, low, grad = torch.zeros_like(p), torch.zeros_like(p), torch.zeros_like(p, dtype=BF16), p.grad
+    written = (p, m, v, low)
+    before = [t._version for t in written]
+    k.fused_adamw_update([p], [grad], [m], [v], step=1, model_params=[low], **HYPER)
+    assert all(t._version > b for t, b in zip(written, before))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    before = grad._version
+    k.global_grad_norm([grad])
+    assert grad._version == before
+    k.clip_grads_by_global_norm([grad], max_norm=1e-3)
+    assert grad._version > before
+
+
 # ---------------------------------------------------------------------------------------------
 # the optimizer
 # ---------------------------------------------------------------------------------------------
@@ -582,6 +614,11 @@ def test_checkpoints_between_widths_and_with_torch(gpu):
     back.load_state_dict(narrow.state_dict())
     want = O.decode(narrow.state[p]["exp_avg_sq"].cpu().numpy(), 3000, "exp_avg_sq")[0]
     O.assert_within(np64(back.state[p]["exp_avg_sq"]), want, 8 * O.U * want + 1e-300, "moment read back")
+    turned = torch.nn.Parameter(p.detach().t().contiguous().t())
+    other = AdamW([turned], lr=1e-3, betas=(0.9, 0.95))
+    other.load_state_dict(narrow.state_dict())
+    assert other.state[turned]["exp_avg_sq"].stride() == turned.stride() != p.stride()
+    assert torch.equal(other.state[turned]["exp_avg_sq"], back.state[p]["exp_avg_sq"])
     theirs.load_state_dict({**saved, "state": {0: {**wide.state_dict()["state"][0], "step": torch.tensor(3.0)}}})
 
 
