@@ -97,8 +97,8 @@ __host__ __device__ __forceinline__ int tensor_of(const L& l, uint32_t b) {
 // ---------------------------------------------------------------------------------------------
 // V values at a time, 4 of float32 or 8 where all types have 16 bits (16 bytes a lane).  Tensors need the alignment of their elements only: the vector types say so, and global
 // loads and stores of any width take such addresses.  A step touches each value once and a list is far larger than the
-// caches, so loads and stores are non-temporal: 268M float32 weights with float32 moments 1395 -> 1294 us (5.4 -> 5.8 TB/s;
-// loads alone 1351, stores alone 1414), the sum of squares of as many values 182 -> 160 us (6.7 TB/s).
+// caches, so loads and stores are non-temporal: 268M float32 weights with float32 moments in chunks of 4096 1395 -> 1294 us
+// (5.4 -> 5.8 TB/s; loads alone 1351, stores alone 1414), the sum of squares of as many values 182 -> 160 us (6.7 TB/s).
 // ---------------------------------------------------------------------------------------------
 template <class T, int V>
 struct Pack {
@@ -180,8 +180,12 @@ __device__ __forceinline__ void adam_value(float& p, float g, float& m, float& v
   p = fmaf(-c.step_size, FAST ? m * __builtin_amdgcn_rcpf(den) : m / den, c.keep * p);
 }
 
-// 32-bit moments.  Each value is read and written once: 28 bytes a value with float32 weights and gradients, about 25
-// operations, so the memory bounds it.
+// 32-bit moments.  Each value is read and written once: 28 bytes a value with float32 weights and gradients, 42
+// instructions, so the memory bounds it: 269M values in 67 tensors take 1187 to 1240 us (6.1 to 6.3 TB/s; a large copy by
+// torch reaches 4.9), 436M with bfloat16 gradients and copies 2.18 ms (5.6 TB/s).  A thread handles one vector of four and
+// a workgroup 1024 values: chunks of 2048 and 4096 (more loads in flight a thread, fewer threads on a CU) take 2 to 4 %
+// longer, 8 values a thread (32-byte pieces of float32) 14 %, workgroups of 128 threads 1 % (odd sizes: 8 %), of 512 and
+// 1024 threads 2 to 6 %; handing each XCD a contiguous range of chunks takes up to 11 % longer.
 constexpr int ADAM_V = 4;
 constexpr int ADAM_CHUNK = NT * ADAM_V;
 
@@ -242,7 +246,10 @@ __global__ __launch_bounds__(NT) void adamw_kernel(AdamArgs<LT> a) {
 //   second moment   v =    s (k / 255)^4   code   k, k = round(255 (v / s)^(1/4)), at least 1 for v > 0
 // Roots space the codes finer towards 0, evenly in relative terms over a range of 1.6e4 in m and 6e4 in sqrt(v); a
 // second moment over 0 never becomes 0, so no update divides by eps alone.  The rounding is to nearest: with stochastic
-// rounding the noise accumulates over 1 / (1 - beta2) steps and updates end up further from the 32-bit ones.
+// rounding the noise accumulates over 1 / (1 - beta2) steps and updates end up further from the 32-bit ones (simulated
+// with gradients whose scales spread as exp(N(0, 0.5)), beta2 = 0.95 / 0.999: 2.3 / 4.9 % of the update to nearest, 3.3 /
+// 6.8 % stochastic; linear codes of m and sqrt(v) 3.2 / 5.7 %, e4m3 8.8 / 17 %, and both of these let small second moments
+// of a wide block become 0).
 // A block whose largest magnitude is below the smallest normal number is stored as 0, one that holds a value that is not
 // finite as NaN.  Codes of places behind the last value are 0.
 // ---------------------------------------------------------------------------------------------
@@ -328,6 +335,12 @@ __device__ __forceinline__ void store_codes(uint8_t* p, Codes<V> codes) {
   __builtin_nontemporal_store(codes, reinterpret_cast<Codes<V>*>(p));
 }
 
+// The step itself: 16.25 bytes a value with float32 weights and gradients, 10.25 with 16-bit ones.  The values of a block
+// sit in neighbouring lanes of one wave, so the new scale is a maximum over registers and three or four lane exchanges,
+// and the moments never leave registers between reading and writing their codes.  269M float32 weights in 683 us (6.4
+// TB/s), 268M bfloat16 ones in 435 us (6.3 TB/s); at first, with correctly rounded roots and quotients, 973 and 923 us,
+// bound by the vector units.  Eight values a lane pay where weights and gradients have 16 bits (435 us; four: 464) and not
+// with float32 (781 against 691 us).
 template <class PT, class GT>
 struct Adam8Shape {
   static constexpr int V = sizeof(PT) == 2 && sizeof(GT) == 2 ? 8 : 4, CHUNK = NT * V;
@@ -393,7 +406,10 @@ __global__ __launch_bounds__(NT) void adamw8_kernel(AdamArgs<LT> a) {
   }
 }
 
-// Conversions between a list of tensors and their 8-bit forms.
+// Conversions between a list of tensors and their 8-bit forms, bound by the memory: 268M values to 8 bits 202 us from
+// float32 (6.7 TB/s) and 131 us from bfloat16 (5.8 to 6.5 TB/s), back to float32 226 us (6.0 TB/s) and to bfloat16 122 us
+// (6.7 TB/s).  These move few bytes a value, so the cost of a workgroup shows (1024 values in one: 20 to 30 % longer):
+// two vectors a thread, four where float32 is written; 128 threads are up to 5 % faster than 256.
 template <class T, bool PACK>
 struct MoveShape {
   static constexpr int V = sizeof(T) == 2 ? 8 : 4, U = sizeof(T) == 4 && !PACK ? 4 : 2, THREADS = 128;
@@ -470,6 +486,9 @@ __device__ __forceinline__ double group_sum(double x) {
   return s;
 }
 
+// Global norm, one read of the list: 872 MB of bfloat16 in 128 us (6.8 TB/s).  Chunks of 16384 values; smaller ones pay for
+// the reduction inside the workgroup (4096: 8 to 14 % longer), larger ones gain nothing.
+//
 // Sum of squares of every chunk, in 64 bits: squares of float32 values neither overflow nor vanish there, and sums over
 // a whole model lose nothing.
 template <class T>
@@ -532,6 +551,8 @@ __global__ __launch_bounds__(THREADS) void norm_finish_kernel(const double* __re
   }
 }
 
+// Scaling: 872 MB of bfloat16 read and written in 287 us (6.1 TB/s).  Reading in the opposite order of the norm, to meet what
+// is left in the caches, changes nothing with or without non-temporal loads.
 template <class T>
 struct ScaleShape {
   static constexpr int V = 16 / sizeof(T), U = 1;
