@@ -116,24 +116,23 @@ class AdamW(WeightDecayMixin, Optimizer):
             # their bytes say nothing about an order of the dimensions, so a checkpoint could not be checked against it
             raise ValueError("8-bit moments need contiguous parameters")
 
+    def _init_param(self, p: torch.Tensor, state: dict) -> None:
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            # the zeros would be part of the graph and every replay would start from them
+            raise RuntimeError("AdamW needs a step before the one that is captured, to make its state")
+        self._check_param(p)
+        state["step"] = self._first_step(p)
+        state["exp_avg"] = self._moment(p)
+        state["exp_avg_sq"] = self._moment(p)
+        if self.master_weights and p.dtype in (torch.bfloat16, torch.float16):
+            state["master"] = p.detach().to(torch.float32)
+
     @torch.no_grad()
     def _init_group(self, group: dict, skip_non_grad_params: bool = True) -> None:
         """Creates the state of every parameter of ``group`` that does not have one yet."""
         for p in group["params"]:
-            if p.grad is None and skip_non_grad_params:
-                continue
-            state = self.state[p]
-            if state:
-                continue
-            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
-                # the zeros would be part of the graph and every replay would start from them
-                raise RuntimeError("AdamW needs a step before the one that is captured, to make its state")
-            self._check_param(p)
-            state["step"] = self._first_step(p)
-            state["exp_avg"] = self._moment(p)
-            state["exp_avg_sq"] = self._moment(p)
-            if self.master_weights and p.dtype in (torch.bfloat16, torch.float16):
-                state["master"] = p.detach().to(torch.float32)
+            if (p.grad is not None or not skip_non_grad_params) and not self.state[p]:
+                self._init_param(p, self.state[p])
 
     @torch.no_grad()
     def step(self, closure: Optional[Callable[[], float]] = None, *, grad_scale: Optional[torch.Tensor] = None) -> Optional[float]:
@@ -148,8 +147,8 @@ class AdamW(WeightDecayMixin, Optimizer):
         if capturing and not self.capturable:
             raise RuntimeError("capturing AdamW.step() needs capturable=True")
         for group in self.param_groups:
-            self._init_group(group)
             batches: dict = {}
+            last = None
             for p in group["params"]:
                 grad = p.grad
                 if grad is None:
@@ -157,22 +156,23 @@ class AdamW(WeightDecayMixin, Optimizer):
                 if grad.is_sparse:
                     raise RuntimeError("AdamW does not support sparse gradients")
                 state = self.state[p]
-                if not self.capturable:
-                    state["step"] += 1
-                key = (p.get_device(), p.dtype, grad.dtype, "master" in state, None if self.capturable else state["step"])
-                batch = batches.get(key)
-                if batch is None:
-                    batch = batches[key] = (self._kernels_take(p, grad), [], [], [])
-                batch[1].append(p)
-                batch[2].append(grad)
-                batch[3].append(state)
+                if not state:
+                    self._init_param(p, state)
+                key = (p.dtype, grad.dtype, p.get_device(), "master" in state, None if self.capturable else state["step"])
+                if key != last:
+                    last = key
+                    if key not in batches:
+                        batches[key] = (self._kernels_take(p, grad), [], [], [])
+                    kernels, params, grads, states = batches[key]
+                params.append(p)
+                grads.append(grad)
+                states.append(state)
             for kernels, params, grads, states in batches.values():
                 if kernels:
                     self._update_batch(params, grads, states, group, grad_scale)
                     continue
                 for p, state in zip(params, states):
-                    if self.capturable:
-                        state["step"] += 1
+                    state["step"] += 1
                     self._update_torch(p, group, grad_scale)
         return None
 
@@ -188,26 +188,33 @@ class AdamW(WeightDecayMixin, Optimizer):
         """One call for parameters of one device, type and step."""
         if not all(map(torch.Tensor.is_contiguous, params)) or not all(map(torch.Tensor.is_contiguous, grads)):
             grads = [g if g.stride() == p.stride() else torch.empty_like(p, dtype=g.dtype).copy_(g) for p, g in zip(params, grads)]
-        step: Any = states[0]["step"]
-        if self.capturable:
-            step = [s["step"] for s in states]
-            torch._foreach_add_(step, 1)
         masters = "master" in states[0]
-        (hip_kernels.fused_adamw_update if self.moment_bits == 32 else hip_kernels.fused_adamw_update_8bit)(
-            [s["master"] for s in states] if masters else params,
-            grads,
-            [s["exp_avg"] for s in states],
-            [s["exp_avg_sq"] for s in states],
-            step=step,
-            lr=group["lr"],
-            beta1=group["betas"][0],
-            beta2=group["betas"][1],
-            eps=group["eps"],
-            weight_decay=group["weight_decay"],
-            weight_decay_method=self.weight_decay_method,
-            grad_scale=grad_scale,
-            model_params=params if masters else None,
-        )
+        steps = [s["step"] for s in states]
+        if self.capturable:
+            torch._foreach_add_(steps, 1)
+        try:
+            (hip_kernels.fused_adamw_update if self.moment_bits == 32 else hip_kernels.fused_adamw_update_8bit)(
+                [s["master"] for s in states] if masters else params,
+                grads,
+                [s["exp_avg"] for s in states],
+                [s["exp_avg_sq"] for s in states],
+                step=steps if self.capturable else steps[0] + 1,
+                lr=group["lr"],
+                beta1=group["betas"][0],
+                beta2=group["betas"][1],
+                eps=group["eps"],
+                weight_decay=group["weight_decay"],
+                weight_decay_method=self.weight_decay_method,
+                grad_scale=grad_scale,
+                model_params=params if masters else None,
+            )
+        except Exception:  # refused before anything was launched: the step does not count
+            if self.capturable:
+                torch._foreach_sub_(steps, 1)
+            raise
+        if not self.capturable:
+            for state in states:
+                state["step"] += 1
 
     def _update_torch(self, p: torch.Tensor, group: dict, grad_scale: Optional[torch.Tensor]) -> None:
         """The update of one parameter as torch statements, in float32 (float64 parameters: in float64)."""

@@ -49,8 +49,11 @@ def clip_grad_norm_(
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     if not grads:
         return torch.tensor(0.0)
-    kernels = len({g.device for g in grads}) == 1 and all(
-        hip_kernels.on_kernel_device(g) and g.dtype in LIST_DTYPES and is_dense(g) for g in grads
+    kernels = (
+        hip_kernels.on_kernel_device(grads[0])
+        and len(set(map(torch.Tensor.get_device, grads))) == 1
+        and {g.dtype for g in grads}.issubset(LIST_DTYPES)
+        and (all(map(torch.Tensor.is_contiguous, grads)) or all(map(is_dense, grads)))
     )
     if kernels and not error_if_nonfinite:
         return hip_kernels.clip_grads_by_global_norm(grads, max_norm=max_norm)

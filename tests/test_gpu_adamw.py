@@ -577,6 +577,28 @@ def test_optimizer_uses_the_kernels_and_matches_its_cpu_statements(gpu, bits, ma
                     assert int(((a - b + 128) % 256 - 128).abs().max()) <= 1  # a code may fall on either side of a border
 
 
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_refused_step_changes_nothing(gpu, capturable):
+    """Two parameters on one piece of memory: the call is refused, steps and moments stay."""
+    flat = torch.ones(100, device=gpu)
+    a, b = torch.nn.Parameter(flat[:60]), torch.nn.Parameter(flat[50:])
+    opt = AdamW([a, b], capturable=capturable)
+    a.grad = torch.ones_like(a)
+    opt.step()
+    kept = flat.clone()
+    b.grad = torch.ones_like(b)
+    a.grad = a.grad.clone()
+    for p in (a, b):
+        opt.state[p] = {} if p is b else opt.state[p]
+    opt.state[b].update({key: (value.clone() if isinstance(value, torch.Tensor) else value) for key, value in opt.state[a].items()})
+    for key in ("exp_avg", "exp_avg_sq"):
+        opt.state[b][key] = torch.zeros_like(b)
+    with pytest.raises(ValueError, match="overlaps"):
+        opt.step()
+    assert float(opt.state[a]["step"]) == float(opt.state[b]["step"]) == 1
+    assert torch.equal(flat, kept) and not opt.state[b]["exp_avg"].any()
+
+
 def test_eight_bit_optimizer_follows_the_32_bit_one(gpu):
     """Twenty steps on the same gradients: the 8-bit updates stay within 10 % of the 32-bit ones (each moment is held
     to half a step, at most 1/127 relative for values near the block's largest and more for small ones)."""
