@@ -95,10 +95,11 @@ __host__ __device__ __forceinline__ int tensor_of(const L& l, uint32_t b) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// V values at a time, 4 of float32 or 8 where all types have 16 bits (16 bytes a lane).  Tensors need the alignment of their elements only: the vector types say so, and global
-// loads and stores of any width take such addresses.  A step touches each value once and a list is far larger than the
-// caches, so loads and stores are non-temporal: 268M float32 weights with float32 moments in chunks of 4096 1395 -> 1294 us
-// (5.4 -> 5.8 TB/s; loads alone 1351, stores alone 1414), the sum of squares of as many values 182 -> 160 us (6.7 TB/s).
+// V values at a time, 4 of float32 or 8 where all types have 16 bits (16 bytes a lane).  Tensors need the alignment of
+// their elements only: the vector types say so, and global loads and stores of any width take such addresses.  A step
+// touches each value once and a list is far larger than the caches, so loads and stores are non-temporal: 268M float32
+// weights with float32 moments in chunks of 4096 1395 -> 1294 us (5.4 -> 5.8 TB/s; loads alone 1351, stores alone 1414),
+// the sum of squares of as many values 182 -> 160 us (6.7 TB/s).  Ten other pairs of cache policies gain nothing on them.
 // ---------------------------------------------------------------------------------------------
 template <class T, int V>
 struct Pack {
@@ -601,9 +602,12 @@ __global__ __launch_bounds__(NT) void scale_list_kernel(ReadList l, ScaleFactor 
   for (int u = 0; u < S::U; ++u) {
     const int e = (u * NT + threadIdx.x) * V;
     if (e >= left) return;
-    const int k = (int)(left - e);
-    if (left - e >= V) store<V>(x + e, load<V>(x + e) * f);
-    else store_part<V>(x + e, load_part<V>(x + e, k) * f, k);
+    if (left - e >= V) {
+      store<V>(x + e, load<V>(x + e) * f);
+    } else {
+      const int k = (int)(left - e);
+      store_part<V>(x + e, load_part<V>(x + e, k) * f, k);
+    }
   }
 }
 

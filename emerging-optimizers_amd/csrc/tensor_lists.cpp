@@ -72,7 +72,13 @@ struct List {
         fast = nullptr;
         refuse(PyExc_TypeError, std::string(who) + ": " + what + "[" + number(i) + "] is not a tensor");
       }
-      t.push_back(&THPVariable_Unpack(items[i]));
+      const at::Tensor& x = THPVariable_Unpack(items[i]);
+      if (x.layout() != at::kStrided || x.is_neg()) {  // values that are not what the memory holds
+        Py_DECREF(fast);
+        fast = nullptr;
+        refuse(PyExc_TypeError, std::string(who) + ": " + what + "[" + number(i) + "] must be a plain strided tensor");
+      }
+      t.push_back(&x);
     }
   }
   List(const List&) = delete;

@@ -244,6 +244,7 @@ int mi_muon_update_bf16(float* param, const float* grad, float* momentum, int64_
  * (model_dtype) of float32 weights, written only.  grad: float32, or the 16-bit type that the weights or their copies
  * have (either one for float32 weights without copies).  exp_avg, exp_avg_sq: the moments m and v, updated in place;
  * moment_bits == 32: float32 values; moment_bits == 8: the 8-bit form described at mi_moments_8bit_pack.
+ * (With 8-bit moments a second moment below 2^-126 counts as 0, in the update too.)
  * t = step (>= 1), or, where step_dev is not NULL, *step_dev[i] for tensor i (float32 on the device).
  * lr_dev: NULL, or a float32 on the device that replaces lr.  grad_scale: NULL (1), or a float32 on the device.
  */

@@ -153,6 +153,22 @@ def test_update_function_refuses(change, exc, text):
         k.fused_adamw_update(**{**HYPER, **lists(**change)})
 
 
+def test_update_function_refuses_what_is_not_a_plain_tensor():
+    for bad, text in (([1.0], "is not a tensor"), (3, "must be a sequence"), ([torch.zeros(4, 6).to_sparse()], "plain strided"),
+                      ([torch.zeros(4, 6, dtype=torch.complex64).conj().imag], "plain strided")):
+        with pytest.raises(TypeError, match=text):
+            k.fused_adamw_update(**{**HYPER, **lists(grads=bad)})
+    with pytest.raises(RuntimeError, match="GPU only"):  # (a step of any number type gets as far as the device)
+        k.fused_adamw_update(**{**HYPER, **lists(), "step": np.int64(3)})
+
+
+def test_a_missing_module_is_an_error(monkeypatch):
+    monkeypatch.setattr(_hip, "_lists", None)
+    monkeypatch.setattr(_hip, "LISTS_PATH", "/nonexistent/_mi_lists.so")
+    with pytest.raises(RuntimeError, match="build it with"):
+        k.fused_adamw_update([], [], [], [], **HYPER)
+
+
 def test_update_functions_take_empty_lists_and_check_packed_moments():
     k.fused_adamw_update([], [], [], [], **HYPER)
     k.fused_adamw_update_8bit([], [], [], [], **HYPER)

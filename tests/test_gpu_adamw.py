@@ -443,6 +443,60 @@ def test_calls_on_two_streams_at_once(gpu):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+def test_calls_follow_the_current_stream(gpu, bits):
+    """On a side stream, behind work that makes the gradients late: the calls wait for it, as everything on that stream."""
+    gen = torch.Generator().manual_seed(18)
+    sizes = [100000, 77]
+    params, grads = values(gen, sizes, 0.02), values(gen, sizes, 1e-3)
+    ms, vs = moments(gen, sizes)
+    if bits == 8:
+        ms, vs = packed_like(ms, "exp_avg"), packed_like(vs, "exp_avg_sq")
+    late = [torch.full_like(g, float("nan")) for g in grads]
+    before = snapshot(params, ms, vs, bits)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        for a, b in zip(late, grads):
+            a.copy_(b)
+        (k.fused_adamw_update if bits == 32 else k.fused_adamw_update_8bit)(params, late, ms, vs, step=4, **HYPER)
+        norm = k.clip_grads_by_global_norm(late, max_norm=1e-3)
+    side.synchronize()
+    check_update(params, grads, ms, vs, before, method="decoupled", step=4, bits=bits)
+    exact = math.sqrt(sum(float((np64(g) ** 2).sum()) for g in grads))
+    assert abs(float(norm) - exact) <= 1.01 * O.U * exact
+
+
+def test_two_graphs_replayed_at_once_share_nothing(gpu):
+    """Norms of two lists, each in a graph of its own, captured on one stream and replayed side by side on two."""
+    gen = torch.Generator().manual_seed(19)
+    lists = [values(gen, [4000000, 77], 1.0), values(gen, [3000000, 99], 3.0)]
+    graphs, norms = [], []
+    k.global_grad_norm(lists[0])
+    torch.cuda.synchronize()
+    for grads in lists:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            norms.append(k.global_grad_norm(grads))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for turn in range(5):
+        for grads in lists:
+            for g in grads:
+                g.mul_(1.5)
+        want = [k.global_grad_norm(grads) for grads in lists]
+        for n in norms:
+            n.zero_()
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for s, graph in zip(streams, graphs):
+                with torch.cuda.stream(s):
+                    graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(norms, want))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 def test_clipped_step_replays_from_a_graph(gpu, bits):
     """Norm, factor and update captured once; each replay equals an eager step on the same gradients."""
     gen = torch.Generator().manual_seed(12)
