@@ -225,11 +225,17 @@ int selftest() {
 
 // Lists of tensors: sizes on both sides of vectors, blocks, chunks and launch limits, more tensors than an argument block
 // holds, sizes past 32 bits; every entry, every combination of types.
-void list_case(const std::vector<int64_t>& sizes, bool quick) {
+// `places`: how many elements behind a line the tensors begin (8-bit moments: 16 bytes each).
+void list_case(const std::vector<int64_t>& sizes, bool quick, int places = 0) {
   const int64_t count = (int64_t)sizes.size();
   const auto lists = [&](int bytes, const char* name) {
     std::vector<void*> p;
-    for (int64_t n : sizes) p.push_back(n ? fake_alloc(bytes ? (size_t)n * bytes : mi_moment_8bit_bytes(n), name) : nullptr);
+    for (int64_t n : sizes) {
+      const size_t skip = (size_t)places * (bytes ? bytes : 16), size = bytes ? (size_t)n * bytes : mi_moment_8bit_bytes(n);
+      char* base = n ? static_cast<char*>(fake_alloc_unregistered(size + skip)) + skip : nullptr;
+      if (base) add_range(base, size, name);
+      p.push_back(base);
+    }
     return p;
   };
   const auto bytes_of = [](int dtype) { return dtype == MI_DTYPE_F32 ? 4 : 2; };
@@ -279,6 +285,10 @@ void list_cases(bool quick) {
   const int64_t launch = (int64_t)1 << 33;  // 2^23 chunks of 1024 values
   list_case({5, launch - 1024, 7, launch, launch + 1, 9, 3 * launch + 77, 11}, quick);
   list_case({((int64_t)1 << 40) - 5}, quick);
+  for (int places : {1, 5, 31, 32, 63}) {
+    list_case({1, 3, 4, 64 - places, 65 - places, 1024 - places, 1025 - places, 1024, 2047, 16384 - places, 16385 - places, 50000}, quick, places);
+    list_case({launch - places, launch, launch + 1, 2 * launch - places}, quick, places);
+  }
 }
 
 int main(int argc, char** argv) {

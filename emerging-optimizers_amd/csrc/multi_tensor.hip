@@ -118,21 +118,40 @@ __device__ __forceinline__ void store(T* p, Floats<V> x) {
   typedef Pack<T, V> X;
   __builtin_nontemporal_store((typename X::at)__builtin_convertvector(x, typename X::type), reinterpret_cast<typename X::at*>(p));
 }
-// The first `k` of V values; zeros for the others.
+// The values [k0, k) of V; zeros for the others.
 template <int V, class T>
-__device__ __forceinline__ Floats<V> load_part(const T* p, int k) {
+__device__ __forceinline__ Floats<V> load_part(const T* p, int k, int k0 = 0) {
   Floats<V> x = {};
 #pragma unroll
   for (int i = 0; i < V; ++i)
-    if (i < k) x[i] = (float)p[i];
+    if (i >= k0 && i < k) x[i] = (float)p[i];
   return x;
 }
 template <int V, class T>
-__device__ __forceinline__ void store_part(T* p, Floats<V> x, int k) {
+__device__ __forceinline__ void store_part(T* p, Floats<V> x, int k, int k0 = 0) {
 #pragma unroll
   for (int i = 0; i < V; ++i)
-    if (i < k) p[i] = (T)x[i];
+    if (i >= k0 && i < k) p[i] = (T)x[i];
 }
+
+// Chunks begin at multiples of 64 elements in memory, not of the tensor: a tensor that begins elsewhere has its first
+// chunk begin that many places before it.  Otherwise the waves of a tensor at an odd place (in a bucket of tensors back to
+// back) share the 128-byte lines at their ends, and lines written in two pieces cost 15 % of a step with 32-bit moments
+// (268M float32 values: 1482 us one element behind a line, 1286 at one), 21 % with 16-bit copies; reading bfloat16 from an
+// odd element costs 27 % of the norm.
+template <class T>
+__host__ __device__ __forceinline__ int places_before(const T* p) {
+  return (int)((uintptr_t)p / sizeof(T) & 63);
+}
+// The part of a vector of V values that a tensor has: [k0, k1) of those at place `at`.
+template <int V>
+struct Part {
+  int k0, k1;
+  __device__ __forceinline__ Part(int64_t at, int64_t n)
+      : k0(at < 0 ? (at > -V ? (int)-at : V) : 0), k1(n - at < V ? (n - at > 0 ? (int)(n - at) : 0) : V) {}
+  __device__ __forceinline__ bool none() const { return k0 >= k1; }
+  __device__ __forceinline__ bool whole() const { return k0 == 0 && k1 == V; }
+};
 
 // ---------------------------------------------------------------------------------------------
 // AdamW
@@ -197,27 +216,26 @@ __global__ __launch_bounds__(NT) void adamw_kernel(AdamArgs<LT> a) {
   const uint32_t chunk = a.list.chunk0 + blockIdx.x;
   const int ti = tensor_of(a.list, chunk);
   const auto t = a.list.t[ti];
-  const int64_t base = (int64_t)(chunk - a.list.first[ti]) * ADAM_CHUNK;
-  PT* __restrict__ p = static_cast<PT*>(t.p) + base;
-  const GT* __restrict__ g = static_cast<const GT*>(t.g) + base;
-  float* __restrict__ m = static_cast<float*>(t.m) + base;
-  float* __restrict__ v = static_cast<float*>(t.v) + base;
-  const int64_t left = t.n - base;
+  // (the moments' places decide; weights and gradients in buckets of the same order have the same ones)
+  const int64_t at = (int64_t)(chunk - a.list.first[ti]) * ADAM_CHUNK - places_before(static_cast<float*>(t.m)) + threadIdx.x * V;
+  const Part<V> part(at, t.n);
   const AdamCoef c = adam_coefficients(a.s, t.step);
-  const int e = threadIdx.x * V;
-  if (e >= left) return;
-  const int k = left - e < V ? (int)(left - e) : V;
+  if (part.none()) return;
+  PT* __restrict__ p = static_cast<PT*>(t.p) + at;
+  const GT* __restrict__ g = static_cast<const GT*>(t.g) + at;
+  float* __restrict__ m = static_cast<float*>(t.m) + at;
+  float* __restrict__ v = static_cast<float*>(t.v) + at;
   F pp, gg, mm, vv;
-  if (k == V) {
-    gg = load<V>(g + e);
-    pp = load<V>(p + e);
-    mm = load<V>(m + e);
-    vv = load<V>(v + e);
+  if (part.whole()) {
+    gg = load<V>(g);
+    pp = load<V>(p);
+    mm = load<V>(m);
+    vv = load<V>(v);
   } else {
-    gg = load_part<V>(g + e, k);
-    pp = load_part<V>(p + e, k);
-    mm = load_part<V>(m + e, k);
-    vv = load_part<V>(v + e, k);
+    gg = load_part<V>(g, part.k1, part.k0);
+    pp = load_part<V>(p, part.k1, part.k0);
+    mm = load_part<V>(m, part.k1, part.k0);
+    vv = load_part<V>(v, part.k1, part.k0);
   }
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -227,16 +245,16 @@ __global__ __launch_bounds__(NT) void adamw_kernel(AdamArgs<LT> a) {
     mm[i] = mi;
     vv[i] = vi;
   }
-  if (k == V) {
-    store<V>(p + e, pp);
-    store<V>(m + e, mm);
-    store<V>(v + e, vv);
-    if constexpr (!__is_same(LT, None)) store<V>(static_cast<LT*>(t.low) + base + e, pp);
+  if (part.whole()) {
+    store<V>(p, pp);
+    store<V>(m, mm);
+    store<V>(v, vv);
+    if constexpr (!__is_same(LT, None)) store<V>(static_cast<LT*>(t.low) + at, pp);
   } else {
-    store_part<V>(p + e, pp, k);
-    store_part<V>(m + e, mm, k);
-    store_part<V>(v + e, vv, k);
-    if constexpr (!__is_same(LT, None)) store_part<V>(static_cast<LT*>(t.low) + base + e, pp, k);
+    store_part<V>(p, pp, part.k1, part.k0);
+    store_part<V>(m, mm, part.k1, part.k0);
+    store_part<V>(v, vv, part.k1, part.k0);
+    if constexpr (!__is_same(LT, None)) store_part<V>(static_cast<LT*>(t.low) + at, pp, part.k1, part.k0);
   }
 }
 
@@ -496,12 +514,12 @@ template <class T>
 __global__ __launch_bounds__(NT) void sumsq_list_kernel(ReadList l, double* __restrict__ partials) {
   const uint32_t chunk = l.chunk0 + blockIdx.x;
   const int ti = tensor_of(l, chunk);
-  const int64_t base = (int64_t)(chunk - l.first[ti]) * NORM_CHUNK;
-  const T* __restrict__ x = static_cast<const T*>(l.t[ti].x) + base;
-  const int64_t left = l.t[ti].n - base;
+  const T* const tensor = static_cast<const T*>(l.t[ti].x);
+  const int64_t base = (int64_t)(chunk - l.first[ti]) * NORM_CHUNK - places_before(tensor), n = l.t[ti].n;
+  const T* __restrict__ x = tensor + base;
   constexpr int V = 16 / sizeof(T);
   double sum = 0.0;
-  if (left >= NORM_CHUNK) {
+  if (base >= 0 && n - base >= NORM_CHUNK) {
 #pragma unroll 4
     for (int e = threadIdx.x * V; e < NORM_CHUNK; e += NT * V) {
       const Floats<V> xx = load<V>(x + e);
@@ -509,8 +527,11 @@ __global__ __launch_bounds__(NT) void sumsq_list_kernel(ReadList l, double* __re
       for (int i = 0; i < V; ++i) sum = fma((double)xx[i], (double)xx[i], sum);
     }
   } else {
-    for (int64_t e = threadIdx.x * V; e < left; e += NT * V) {
-      const Floats<V> xx = left - e >= V ? load<V>(x + e) : load_part<V>(x + e, (int)(left - e));
+#pragma unroll 2
+    for (int e = threadIdx.x * V; e < NORM_CHUNK; e += NT * V) {
+      const Part<V> part(base + e, n);
+      if (part.none()) continue;
+      const Floats<V> xx = part.whole() ? load<V>(x + e) : load_part<V>(x + e, part.k1, part.k0);
 #pragma unroll
       for (int i = 0; i < V; ++i) sum = fma((double)xx[i], (double)xx[i], sum);
     }
@@ -556,8 +577,7 @@ __global__ __launch_bounds__(THREADS) void norm_finish_kernel(const double* __re
 // is left in the caches, changes nothing with or without non-temporal loads.
 template <class T>
 struct ScaleShape {
-  static constexpr int V = 16 / sizeof(T), U = 1;
-  static constexpr int CHUNK = NT * V * U;
+  static constexpr int V = 16 / sizeof(T), CHUNK = NT * V;
 };
 
 // x <- factor x; a factor of 1 changes nothing and reads nothing.  The factor is *factor, or, with FINISH, what the
@@ -595,20 +615,13 @@ __global__ __launch_bounds__(NT) void scale_list_kernel(ReadList l, ScaleFactor 
   if (f == 1.0f) return;
   const uint32_t chunk = l.chunk0 + blockIdx.x;
   const int ti = tensor_of(l, chunk);
-  const int64_t base = (int64_t)(chunk - l.first[ti]) * S::CHUNK;
-  T* __restrict__ x = static_cast<T*>(const_cast<void*>(l.t[ti].x)) + base;
-  const int64_t left = l.t[ti].n - base;
-#pragma unroll
-  for (int u = 0; u < S::U; ++u) {
-    const int e = (u * NT + threadIdx.x) * V;
-    if (e >= left) return;
-    if (left - e >= V) {
-      store<V>(x + e, load<V>(x + e) * f);
-    } else {
-      const int k = (int)(left - e);
-      store_part<V>(x + e, load_part<V>(x + e, k) * f, k);
-    }
-  }
+  T* const tensor = static_cast<T*>(const_cast<void*>(l.t[ti].x));
+  const int64_t at = (int64_t)(chunk - l.first[ti]) * S::CHUNK - places_before(tensor) + threadIdx.x * V;
+  const Part<V> part(at, l.t[ti].n);
+  if (part.none()) return;
+  T* __restrict__ x = tensor + at;
+  if (part.whole()) store<V>(x, load<V>(x) * f);
+  else store_part<V>(x, load_part<V>(x, part.k1, part.k0) * f, part.k1, part.k0);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -616,22 +629,23 @@ __global__ __launch_bounds__(NT) void scale_list_kernel(ReadList l, ScaleFactor 
 // ---------------------------------------------------------------------------------------------
 // Walks a list of tensors and hands full argument blocks to `launch(list, chunks)`: empty tensors are left out, a block
 // ends when it is full or its chunks would be too many, and a tensor with too many of them has launches of its own.
-// `fill(i)` makes the entry of tensor i.
-template <class L, class Fill, class Launch>
-int for_each_list(int64_t count, const int64_t* numel, int64_t chunk, L& list, Fill fill, Launch launch) {
+// `fill(i)` makes the entry of tensor i, `before(entry)` says how many places before the tensor its first chunk begins.
+template <class L, class Fill, class Before, class Launch>
+int for_each_list(int64_t count, const int64_t* numel, int64_t chunk, L& list, Fill fill, Before before, Launch launch) {
   int64_t chunks = 0;
   list.count = 0;
   list.chunk0 = 0;
   for (int64_t i = 0; i < count; ++i) {
     if (numel[i] == 0) continue;
-    const int64_t c = (numel[i] + chunk - 1) / chunk;
+    const auto entry = fill(i);
+    const int64_t c = (numel[i] + before(entry) + chunk - 1) / chunk;
     if (list.count == L::CAPACITY || (list.count > 0 && chunks + c > MAX_CHUNKS)) {
       if (int rc = launch(list, chunks)) return rc;
       list.count = 0;
       chunks = 0;
     }
     list.first[list.count] = (uint32_t)chunks;
-    list.t[list.count++] = fill(i);
+    list.t[list.count++] = entry;
     chunks += c;
     if (chunks > MAX_CHUNKS) {
       for (int64_t at = 0; at < c; at += MAX_CHUNKS) {
@@ -646,21 +660,33 @@ int for_each_list(int64_t count, const int64_t* numel, int64_t chunk, L& list, F
   return list.count ? launch(list, chunks) : MI_OK;
 }
 
+constexpr auto at_tensor = [](const auto&) { return 0; };  // chunks begin with the tensor
+// Chunks begin at multiples of 64 elements (places_before).
+template <class T>
+constexpr auto at_line_of = [](const ReadTensor& t) { return places_before(static_cast<const T*>(t.x)); };
+
 int launched(const char* who) {
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MI_OK : fail(MI_ERR_LAUNCH, "%s: launch failed: %s", who, hipGetErrorString(e));
 }
 
 #ifdef MI_HOST_CHECK
-// Every chunk of a launch falls into the tensor the bisection finds, at an offset inside it.
-template <class L>
-void walk(const L& l, int64_t chunks, int64_t chunk) {
+// Every chunk of a launch falls into the tensor the bisection finds and reaches into it, and the chunks of a tensor
+// reach its end (those of a tensor with launches of its own are walked launch by launch).
+template <class L, class Before>
+void walk(const L& l, int64_t chunks, int64_t chunk, Before before) {
   for (int64_t i = 0; i < chunks; i += (chunks > 4096 && i > 64 && i < chunks - 64) ? 61 : 1) {
     const int64_t b = l.chunk0 + i;
     const int ti = tensor_of(l, (uint32_t)b);
     if (b >> 32) host_check::fail("a chunk number past 32 bits");
     if (ti < 0 || ti >= l.count || l.first[ti] > b) host_check::fail("a chunk without a tensor");
-    else if ((b - l.first[ti]) * chunk >= l.t[ti].n) host_check::fail("a chunk behind the end of its tensor");
+    else if ((b - l.first[ti]) * chunk - before(l.t[ti]) >= l.t[ti].n) host_check::fail("a chunk behind the end of its tensor");
+    else if ((b - l.first[ti] + 1) * chunk - before(l.t[ti]) <= 0) host_check::fail("a chunk before the start of its tensor");
+  }
+  for (int i = 0; i < l.count; ++i) {
+    const int64_t end = i + 1 < l.count ? l.first[i + 1] : l.chunk0 + chunks;
+    const bool last = i + 1 < l.count || chunks < MAX_CHUNKS;
+    if (last && (end - l.first[i]) * chunk - before(l.t[i]) < l.t[i].n) host_check::fail("chunks that end before their tensor");
   }
 }
 #define MI_WALK(...) walk(__VA_ARGS__)
@@ -803,9 +829,10 @@ int adam_impl(int64_t count, void* const* param, const void* const* grad, void* 
   if (!step_dev) bias_terms(s.ln_b1, s.ln_b2, step, lr, &s.step_size, &s.inv_sqrt_bc2);
   const int64_t chunk = !bits8 ? ADAM_CHUNK : pb == 2 && gb == 2 ? Adam8Shape<__bf16, __bf16>::CHUNK : Adam8Shape<float, float>::CHUNK;
   const auto entry = [&](int64_t i) { return AdamTensor{param[i], grad[i], exp_avg[i], exp_avg_sq[i], step_dev ? step_dev[i] : nullptr, numel[i]}; };
+  const auto before = [&](const AdamTensor& t) { return bits8 ? 0 : places_before(static_cast<float*>(t.m)); };
   const auto state_footprints = [&](const auto& l, int64_t chunks) {
     MI_OTHER_LAUNCH();
-    MI_WALK(l, chunks, chunk);
+    MI_WALK(l, chunks, chunk, before);
     for (int i = 0; i < l.count; ++i) {
       [[maybe_unused]] const AdamTensor& t = l.t[i];
       [[maybe_unused]] const int64_t moment = bits8 ? (int64_t)mi_moment_8bit_bytes(t.n) : t.n;
@@ -819,7 +846,7 @@ int adam_impl(int64_t count, void* const* param, const void* const* grad, void* 
     const auto run = [&](auto* a, auto launch) {
       a->s = s;
       return for_each_list(
-          count, numel, chunk, a->list, [&](int64_t i) { return AdamTensorCopy{entry(i), model_param[i]}; },
+          count, numel, chunk, a->list, [&](int64_t i) { return AdamTensorCopy{entry(i), model_param[i]}; }, before,
           [&](const auto& l, int64_t chunks) -> int {
             state_footprints(l, chunks);
             for (int i = 0; i < l.count; ++i) MI_FOOTPRINT("16-bit copy", l.t[i].low, 2, 1, 0, 1, l.t[i].n, l.t[i].n);
@@ -835,7 +862,7 @@ int adam_impl(int64_t count, void* const* param, const void* const* grad, void* 
   }
   AdamArgs<None> a;
   a.s = s;
-  return for_each_list(count, numel, chunk, a.list, entry, [&](const auto& l, int64_t chunks) -> int {
+  return for_each_list(count, numel, chunk, a.list, entry, before, [&](const auto& l, int64_t chunks) -> int {
     state_footprints(l, chunks);
     if (param_dtype == MI_DTYPE_F32) return adam_launch_grad<float, None>(grad_dtype, bits8, a, chunks, stream);
     if (param_dtype == MI_DTYPE_BF16) return adam_launch_grad<__bf16, None>(grad_dtype, bits8, a, chunks, stream);
@@ -855,9 +882,10 @@ int for_each_type(int64_t count, const int* dtype, Body body) {
   return MI_OK;
 }
 
+// Chunks of a list at most, wherever its tensors begin.
 int64_t norm_chunks(int64_t count, const int64_t* numel) {
   int64_t chunks = 0;
-  for (int64_t i = 0; i < count; ++i) chunks += (numel[i] + NORM_CHUNK - 1) / NORM_CHUNK;
+  for (int64_t i = 0; i < count; ++i) chunks += numel[i] ? (numel[i] + 63 + NORM_CHUNK - 1) / NORM_CHUNK : 0;
   return chunks;
 }
 
@@ -872,33 +900,36 @@ int check_list(const char* who, int64_t count, const void* const* x, const int64
   return MI_OK;
 }
 
-// Partial sums of squares of a list.
+// Partial sums of squares of a list, *total of them.
 int sumsq_impl(const char* who, int64_t count, const void* const* x, const int64_t* numel, const int* dtype, double max_norm, double* partials,
                size_t partials_len, float* out, int64_t* total, hipStream_t stream) {
   if (int rc = check_list(who, count, x, numel, dtype)) return rc;
   if (!out) return fail(MI_ERR_BAD_ARG, "%s: no output", who);
   if (!(max_norm >= 0.0)) return fail(MI_ERR_BAD_ARG, "%s: max_norm must not be negative", who);
-  *total = norm_chunks(count, numel);
-  if (*total > 0 && (!partials || partials_len < (size_t)*total))
-    return fail(MI_ERR_WORKSPACE, "%s: %lld partial sums are needed", who, (long long)*total);
-  MI_FOOTPRINT("partial sums", partials, 8, 1, 0, 1, *total, *total);
+  const int64_t most = norm_chunks(count, numel);
+  if (most > 0 && (!partials || partials_len < (size_t)most))
+    return fail(MI_ERR_WORKSPACE, "%s: %lld partial sums are needed", who, (long long)most);
   MI_FOOTPRINT("norm and factor", out, 4, 1, 0, 1, 2, 2);
-  int64_t done = 0;
+  int64_t& done = *total;
+  done = 0;
   ReadList l;
   return for_each_type(count, dtype, [&](int64_t at, int64_t len, int dt) {
-    return for_each_list(
-        len, numel + at, NORM_CHUNK, l, [&](int64_t i) { return ReadTensor{x[at + i], numel[at + i]}; },
-        [&](const ReadList& list, int64_t chunks) -> int {
-          MI_OTHER_LAUNCH();
-          MI_WALK(list, chunks, NORM_CHUNK);
-          for (int i = 0; i < list.count; ++i) MI_FOOTPRINT("tensor", list.t[i].x, element_bytes(dt), 1, 0, 1, list.t[i].n, list.t[i].n);
-          const dim3 grid((unsigned)chunks), block(NT);
-          if (dt == MI_DTYPE_F32) hipLaunchKernelGGL(sumsq_list_kernel<float>, grid, block, 0, stream, list, partials + done);
-          else if (dt == MI_DTYPE_BF16) hipLaunchKernelGGL(sumsq_list_kernel<__bf16>, grid, block, 0, stream, list, partials + done);
-          else hipLaunchKernelGGL(sumsq_list_kernel<_Float16>, grid, block, 0, stream, list, partials + done);
-          done += chunks;
-          return launched(who);
-        });
+    const auto run = [&](auto before, auto kernel) {
+      return for_each_list(
+          len, numel + at, NORM_CHUNK, l, [&](int64_t i) { return ReadTensor{x[at + i], numel[at + i]}; }, before,
+          [&](const ReadList& list, int64_t chunks) -> int {
+            MI_OTHER_LAUNCH();
+            MI_WALK(list, chunks, NORM_CHUNK, before);
+            MI_FOOTPRINT("partial sums", partials + done, 8, 1, 0, 1, chunks, chunks);
+            for (int i = 0; i < list.count; ++i) MI_FOOTPRINT("tensor", list.t[i].x, element_bytes(dt), 1, 0, 1, list.t[i].n, list.t[i].n);
+            hipLaunchKernelGGL(kernel, dim3((unsigned)chunks), dim3(NT), 0, stream, list, partials + done);
+            done += chunks;
+            return launched(who);
+          });
+    };
+    if (dt == MI_DTYPE_F32) return run(at_line_of<float>, sumsq_list_kernel<float>);
+    if (dt == MI_DTYPE_BF16) return run(at_line_of<__bf16>, sumsq_list_kernel<__bf16>);
+    return run(at_line_of<_Float16>, sumsq_list_kernel<_Float16>);
   });
 }
 
@@ -924,19 +955,20 @@ template <bool FINISH>
 int scale_launches(const char* who, int64_t count, void* const* x, const int64_t* numel, const int* dtype, const ScaleFactor& sf, hipStream_t stream) {
   ReadList l;
   return for_each_type(count, dtype, [&](int64_t at, int64_t len, int dt) {
-    const int64_t chunk = dt == MI_DTYPE_F32 ? ScaleShape<float>::CHUNK : ScaleShape<__bf16>::CHUNK;
-    return for_each_list(
-        len, numel + at, chunk, l, [&](int64_t i) { return ReadTensor{x[at + i], numel[at + i]}; },
-        [&](const ReadList& list, int64_t chunks) -> int {
-          MI_OTHER_LAUNCH();
-          MI_WALK(list, chunks, chunk);
-          for (int i = 0; i < list.count; ++i) MI_FOOTPRINT("tensor", list.t[i].x, element_bytes(dt), 1, 0, 1, list.t[i].n, list.t[i].n);
-          const dim3 grid((unsigned)chunks), block(NT);
-          if (dt == MI_DTYPE_F32) hipLaunchKernelGGL((scale_list_kernel<float, FINISH>), grid, block, 0, stream, list, sf);
-          else if (dt == MI_DTYPE_BF16) hipLaunchKernelGGL((scale_list_kernel<__bf16, FINISH>), grid, block, 0, stream, list, sf);
-          else hipLaunchKernelGGL((scale_list_kernel<_Float16, FINISH>), grid, block, 0, stream, list, sf);
-          return launched(who);
-        });
+    const auto run = [&](int64_t chunk, auto before, auto kernel) {
+      return for_each_list(
+          len, numel + at, chunk, l, [&](int64_t i) { return ReadTensor{x[at + i], numel[at + i]}; }, before,
+          [&](const ReadList& list, int64_t chunks) -> int {
+            MI_OTHER_LAUNCH();
+            MI_WALK(list, chunks, chunk, before);
+            for (int i = 0; i < list.count; ++i) MI_FOOTPRINT("tensor", list.t[i].x, element_bytes(dt), 1, 0, 1, list.t[i].n, list.t[i].n);
+            hipLaunchKernelGGL(kernel, dim3((unsigned)chunks), dim3(NT), 0, stream, list, sf);
+            return launched(who);
+          });
+    };
+    if (dt == MI_DTYPE_F32) return run(ScaleShape<float>::CHUNK, at_line_of<float>, scale_list_kernel<float, FINISH>);
+    if (dt == MI_DTYPE_BF16) return run(ScaleShape<__bf16>::CHUNK, at_line_of<__bf16>, scale_list_kernel<__bf16, FINISH>);
+    return run(ScaleShape<_Float16>::CHUNK, at_line_of<_Float16>, scale_list_kernel<_Float16, FINISH>);
   });
 }
 
@@ -995,10 +1027,10 @@ int move_impl(bool pack, int64_t count, const void* const* src, void* const* dst
   static_assert(MoveShape<__bf16, true>::CHUNK == MoveShape<__bf16, false>::CHUNK, "one chunk for both directions");
   MoveList l;
   return for_each_list(
-      count, numel, chunk, l, [&](int64_t i) { return MoveTensor{src[i], dst[i], numel[i]}; },
+      count, numel, chunk, l, [&](int64_t i) { return MoveTensor{src[i], dst[i], numel[i]}; }, at_tensor,
       [&](const MoveList& list, int64_t chunks) -> int {
         MI_OTHER_LAUNCH();
-        MI_WALK(list, chunks, chunk);
+        MI_WALK(list, chunks, chunk, at_tensor);
         for (int i = 0; i < list.count; ++i) {
           [[maybe_unused]] const MoveTensor& t = list.t[i];
           [[maybe_unused]] const int64_t bytes8 = (int64_t)mi_moment_8bit_bytes(t.n);
