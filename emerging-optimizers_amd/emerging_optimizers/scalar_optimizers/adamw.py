@@ -5,7 +5,8 @@ All parameters of one kind are updated by one multi-tensor call (``hip_kernels.f
 ``torch.optim.AdamW``; the defaults and the names of the state's entries are those of that class, so checkpoints move
 in both directions.  Weight decay has the methods of the other optimizers of this package.
 
-On the CPU, on GPUs other than gfx950 and for float64 parameters the same formulas run as torch statements.
+On the CPU, on GPUs other than gfx950, for float64 parameters and for a bfloat16 parameter with a float16 gradient (or the
+other way round) the same formulas run as torch statements.
 """
 
 from __future__ import annotations
