@@ -527,10 +527,10 @@ __global__ __launch_bounds__(NT) void sumsq_list_kernel(ReadList l, double* __re
       for (int i = 0; i < V; ++i) sum = fma((double)xx[i], (double)xx[i], sum);
     }
   } else {
-#pragma unroll 2
-    for (int e = threadIdx.x * V; e < NORM_CHUNK; e += NT * V) {
+    const int end = n - base < NORM_CHUNK ? (int)(n - base) : NORM_CHUNK;
+#pragma unroll 4
+    for (int e = threadIdx.x * V; e < end; e += NT * V) {
       const Part<V> part(base + e, n);
-      if (part.none()) continue;
       const Floats<V> xx = part.whole() ? load<V>(x + e) : load_part<V>(x + e, part.k1, part.k0);
 #pragma unroll
       for (int i = 0; i < V; ++i) sum = fma((double)xx[i], (double)xx[i], sum);
