@@ -359,12 +359,15 @@ def _moments_plain(state):
 # the kernels
 # ---------------------------------------------------------------------------------------------
 def _kernels():
-    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "emerging-optimizers_amd")
-    if path not in sys.path:
-        sys.path.insert(1, path)
-    from emerging_optimizers import hip_kernels
+    """The framework's operators, imported once as a program does."""
+    if not hasattr(_kernels, "module"):
+        path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "emerging-optimizers_amd")
+        if path not in sys.path:
+            sys.path.insert(1, path)
+        from emerging_optimizers import hip_kernels
 
-    return hip_kernels
+        _kernels.module = hip_kernels
+    return _kernels.module
 
 
 def _adamw_own(state, k):
