@@ -50,12 +50,20 @@ std::string text_of(at::IntArrayRef v) {
 // The elements fill one block of memory, in whatever order of the dimensions.
 bool is_dense(const at::Tensor& t) { return t.is_contiguous() || t.is_non_overlapping_and_dense(); }
 
-// Tensors of a Python sequence; the sequence keeps them alive during the call.
+// Tensors of a Python sequence; the sequence keeps them alive during the call.  What the checks ask of a tensor is read
+// once, into a small record.
+struct Item {
+  const at::Tensor* t;
+  int64_t n;
+  at::ScalarType type;
+  int gpu;  // -1: not on a GPU
+  bool contiguous;
+};
 struct List {
   const char* who;
   const char* what;
   PyObject* fast = nullptr;
-  std::vector<const at::Tensor*> t;
+  std::vector<Item> items;
 
   List(const char* who_, const char* what_, PyObject* sequence) : who(who_), what(what_) {
     fast = PySequence_Fast(sequence, "");
@@ -64,41 +72,37 @@ struct List {
       refuse(PyExc_TypeError, std::string(who) + ": " + what + " must be a sequence of tensors");
     }
     const Py_ssize_t n = PySequence_Fast_GET_SIZE(fast);
-    PyObject** items = PySequence_Fast_ITEMS(fast);
-    t.reserve(n);
-    for (Py_ssize_t i = 0; i < n; ++i) {
-      if (!THPVariable_Check(items[i])) {
-        Py_DECREF(fast);
-        fast = nullptr;
-        refuse(PyExc_TypeError, std::string(who) + ": " + what + "[" + number(i) + "] is not a tensor");
+    PyObject** objects = PySequence_Fast_ITEMS(fast);
+    try {
+      items.reserve(n);
+      for (Py_ssize_t i = 0; i < n; ++i) {
+        if (!THPVariable_Check(objects[i])) refuse(PyExc_TypeError, at_(i) + " is not a tensor");
+        const at::Tensor& x = THPVariable_Unpack(objects[i]);
+        // (values that are not what the memory holds)
+        if (x.layout() != at::kStrided || x.is_neg()) refuse(PyExc_TypeError, at_(i) + " must be a plain strided tensor");
+        items.push_back({&x, x.numel(), x.scalar_type(), x.is_cuda() ? (int)x.get_device() : -1, x.is_contiguous()});
       }
-      const at::Tensor& x = THPVariable_Unpack(items[i]);
-      if (x.layout() != at::kStrided || x.is_neg()) {  // values that are not what the memory holds
-        Py_DECREF(fast);
-        fast = nullptr;
-        refuse(PyExc_TypeError, std::string(who) + ": " + what + "[" + number(i) + "] must be a plain strided tensor");
-      }
-      t.push_back(&x);
+    } catch (...) {
+      Py_DECREF(fast);
+      throw;
     }
   }
   List(const List&) = delete;
   List& operator=(const List&) = delete;
   ~List() { Py_XDECREF(fast); }
 
-  int64_t size() const { return (int64_t)t.size(); }
-  const at::Tensor& operator[](size_t i) const { return *t[i]; }
+  int64_t size() const { return (int64_t)items.size(); }
+  const at::Tensor& operator[](size_t i) const { return *items[i].t; }
   std::string at_(size_t i) const { return std::string(who) + ": " + what + "[" + number((int64_t)i) + "]"; }
 
   // The one data type of the list, out of those whose bit is set (bit c for type code c).
   int dtype(int allowed) const {
-    bool ok = !t.empty();
-    for (const at::Tensor* x : t) {
-      const int c = dtype_code(x->scalar_type());
-      ok = ok && c >= 0 && (allowed >> c & 1) && x->scalar_type() == t[0]->scalar_type();
-    }
-    if (ok) return dtype_code(t[0]->scalar_type());
+    const int code = items.empty() ? -1 : dtype_code(items[0].type);
+    bool ok = code >= 0 && (allowed >> code & 1);
+    for (const Item& x : items) ok = ok && x.type == items[0].type;
+    if (ok) return code;
     std::vector<std::string> found;
-    for (const at::Tensor* x : t) found.push_back(dtype_name(x->scalar_type()));
+    for (const Item& x : items) found.push_back(dtype_name(x.type));
     std::sort(found.begin(), found.end());
     found.erase(std::unique(found.begin(), found.end()), found.end());
     std::string names, options;
@@ -111,54 +115,54 @@ struct List {
   // Shapes and memory order of another list, whose tensors' elements fill their memory.
   void like(const List& o) const {
     if (size() != o.size()) refuse(PyExc_ValueError, std::string(who) + ": " + number(size()) + " " + what + " for " + number(o.size()) + " " + o.what);
-    for (size_t i = 0; i < t.size(); ++i) {
-      const at::Tensor &x = *t[i], &p = *o.t[i];
+    for (size_t i = 0; i < items.size(); ++i) {
+      const at::Tensor &x = *items[i].t, &p = *o.items[i].t;
       if (!x.sizes().equals(p.sizes()))
         refuse(PyExc_ValueError, at_(i) + " has shape " + text_of(x.sizes()) + ", its param " + text_of(p.sizes()));
-      if (x.is_contiguous() && p.is_contiguous()) continue;
+      if (items[i].contiguous && o.items[i].contiguous) continue;
       if (!x.strides().equals(p.strides()) || !is_dense(p))
         refuse(PyExc_ValueError, at_(i) + " must fill its memory in the order of its param, got strides " + text_of(x.strides()) + " and " + text_of(p.strides()));
     }
   }
 
   void dense() const {
-    for (const at::Tensor* x : t)
-      if (!is_dense(*x)) refuse(PyExc_ValueError, std::string(who) + ": " + what + " must fill their memory");
+    for (const Item& x : items)
+      if (!x.contiguous && !is_dense(*x.t)) refuse(PyExc_ValueError, std::string(who) + ": " + what + " must fill their memory");
   }
 
   // 8-bit forms of the moments of another list.
   void packed(const List& o) const {
     if (size() != o.size()) refuse(PyExc_ValueError, std::string(who) + ": " + number(size()) + " " + what + " for " + number(o.size()) + " tensors");
-    for (size_t i = 0; i < t.size(); ++i) {
-      if (t[i]->scalar_type() != at::kByte) refuse(PyExc_TypeError, at_(i) + " must be uint8, got " + dtype_name(t[i]->scalar_type()));
-      const int64_t want = (int64_t)mi_moment_8bit_bytes(o[i].numel());
-      if (t[i]->numel() != want || !t[i]->is_contiguous())
-        refuse(PyExc_ValueError, at_(i) + " must be " + number(want) + " contiguous bytes, got " + text_of(t[i]->sizes()));
+    for (size_t i = 0; i < items.size(); ++i) {
+      if (items[i].type != at::kByte) refuse(PyExc_TypeError, at_(i) + " must be uint8, got " + dtype_name(items[i].type));
+      const int64_t want = (int64_t)mi_moment_8bit_bytes(o.items[i].n);
+      if (items[i].n != want || !items[i].contiguous)
+        refuse(PyExc_ValueError, at_(i) + " must be " + number(want) + " contiguous bytes, got " + text_of((*this)[i].sizes()));
     }
   }
 
   std::vector<void*> pointers() const {
-    std::vector<void*> p(t.size());
-    for (size_t i = 0; i < t.size(); ++i) p[i] = t[i]->data_ptr();
+    std::vector<void*> p(items.size());
+    for (size_t i = 0; i < items.size(); ++i) p[i] = items[i].t->data_ptr();
     return p;
   }
   // The call writes these tensors: autograd's version counters move as after an in-place operation, so a backward pass
   // over a graph that saved one of them is refused.
   void written() const {
-    for (const at::Tensor* x : t)
-      if (!x->is_inference()) x->unsafeGetTensorImpl()->bump_version();
+    for (const Item& x : items)
+      if (x.t->unsafeGetTensorImpl()->version_counter().enabled()) x.t->unsafeGetTensorImpl()->bump_version();
   }
   std::vector<int64_t> numels() const {
-    std::vector<int64_t> n(t.size());
-    for (size_t i = 0; i < t.size(); ++i) n[i] = t[i]->numel();
+    std::vector<int64_t> n(items.size());
+    for (size_t i = 0; i < items.size(); ++i) n[i] = items[i].n;
     return n;
   }
   // Data types of the list, which may differ.
   std::vector<int> dtypes() const {
-    std::vector<int> d(t.size());
-    for (size_t i = 0; i < t.size(); ++i) {
-      d[i] = dtype_code(t[i]->scalar_type());
-      if (d[i] < 0) refuse(PyExc_TypeError, std::string(who) + ": " + what + " must be float32, bfloat16 or float16, got " + dtype_name(t[i]->scalar_type()));
+    std::vector<int> d(items.size());
+    for (size_t i = 0; i < items.size(); ++i) {
+      d[i] = dtype_code(items[i].type);
+      if (d[i] < 0) refuse(PyExc_TypeError, std::string(who) + ": " + what + " must be float32, bfloat16 or float16, got " + dtype_name(items[i].type));
     }
     return d;
   }
@@ -166,17 +170,16 @@ struct List {
 
 // The one GPU all tensors of the lists are on.
 c10::Device one_gpu(const char* who, std::initializer_list<const List*> lists) {
-  c10::Device device(c10::kCPU);
+  int gpu = -1;
   for (const List* l : lists) {
     if (!l) continue;
-    for (const at::Tensor* x : l->t) {
-      if (!x->is_cuda()) refuse(PyExc_RuntimeError, std::string(who) + " runs on the GPU only; got a tensor on " + x->device().str());
-      if (device.is_cpu()) device = x->device();
-      else if (x->device() != device)
-        refuse(PyExc_ValueError, std::string(who) + ": all tensors of a call must be on one GPU, got " + device.str() + " and " + x->device().str());
+    for (const Item& x : l->items) {
+      if (x.gpu < 0) refuse(PyExc_RuntimeError, std::string(who) + " runs on the GPU only; got a tensor on " + x.t->device().str());
+      if (gpu < 0) gpu = x.gpu;
+      if (x.gpu != gpu) refuse(PyExc_ValueError, std::string(who) + ": all tensors of a call must be on one GPU, got numbers " + number(gpu) + " and " + number(x.gpu));
     }
   }
-  return device;
+  return gpu < 0 ? c10::Device(c10::kCPU) : c10::Device(c10::kCUDA, (c10::DeviceIndex)gpu);
 }
 
 const at::Tensor& device_scalar(const char* who, const char* what, PyObject* o, c10::Device device, const char* like) {

@@ -576,6 +576,9 @@ def test_autograd_notices_what_the_calls_write(gpu):
     assert all(t._version > b for t, b in zip(written, before))
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+    with torch.inference_mode():  # (tensors without a counter)
+        lists = [[torch.ones(10, device=gpu)] for _ in range(4)]
+    k.fused_adamw_update(*lists, step=1, **HYPER)
     before = grad._version
     k.global_grad_norm([grad])
     assert grad._version == before
