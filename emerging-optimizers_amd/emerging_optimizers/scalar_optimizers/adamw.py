@@ -66,7 +66,8 @@ class AdamW(WeightDecayMixin, Optimizer):
         moment_bits: 32 for float32 moments, 8 for one byte a value and a float32 scale for each 64 values
             (``hip_kernels.pack_moments_8bit``); 8 saves 5.9 bytes a parameter, and updates differ from the 32-bit
             ones by a few per cent
-        master_weights: keep float32 weights of record for 16-bit parameters (in the state, as ``master``)
+        master_weights: keep float32 weights of record for 16-bit parameters (in the state, as ``master``); without them
+            a step smaller than half the distance between neighbouring 16-bit numbers is lost
         capturable: keep the step count on the GPU, so that a captured ``step()`` counts on when it is replayed
     """
 

@@ -280,6 +280,7 @@ int mi_scale_tensors(int64_t count, void* const* x, const int64_t* numel, const 
  * magnitude of the block.
  *   first moment:  code k in -127 .. 127 stands for sign(k) s (k / 127)^2; |k| = round(127 sqrt(|m| / s))
  *   second moment: code k in 0 .. 255 stands for s (k / 255)^4; k = round(255 (v / s)^(1/4)), at least 1 for v > 0
+ * (A value that float32 rounding puts on either side of a border between two codes may take either of them.)
  * A block with a value that is not finite stands for NaN throughout (s = NaN), one whose largest magnitude is below
  * 2^-126 for 0; codes behind the last value are 0.  pack writes the form of float32, bfloat16 or float16 values
  * (dtype), unpack the values that a form stands for.  second_moment: 0 or 1.
