@@ -202,7 +202,7 @@ __device__ __forceinline__ void adam_value(float& p, float g, float& m, float& v
 
 // 32-bit moments.  Each value is read and written once: 28 bytes a value with float32 weights and gradients, 42
 // instructions, so the memory bounds it: 269M values in 67 tensors take 1187 to 1240 us (6.1 to 6.3 TB/s; a large copy by
-// torch reaches 4.9), 436M with bfloat16 gradients and copies 2.18 ms (5.6 TB/s).  A thread handles one vector of four and
+// torch reaches 4.9), 436M with bfloat16 gradients and copies 2.09 ms (5.8 TB/s).  A thread handles one vector of four and
 // a workgroup 1024 values: chunks of 2048 and 4096 (more loads in flight a thread, fewer threads on a CU) take 2 to 4 %
 // longer, 8 values a thread (32-byte pieces of float32) 14 %, workgroups of 128 threads 1 % (odd sizes: 8 %), of 512 and
 // 1024 threads 2 to 6 %; handing each XCD a contiguous range of chunks takes up to 11 % longer.
@@ -759,11 +759,22 @@ int check_numel(const char* who, int64_t count, const int64_t* numel) {
   return MI_OK;
 }
 
+// LDS that a workgroup of the step with 32-bit moments holds without using it, so that fewer than eight of them share a CU:
+// with seven or eight streams of two element sizes in flight, the memory does better with fewer rows open at once.  With
+// 16-bit copies five workgroups (436M values in 19 tensors: 2280 us a clipped step with eight, 2251 with seven, 2216 with
+// six, 2197 with five and four), with 16-bit weights alone six (268M: 970 us with eight, 936 with six, 942 with five); with
+// float32 throughout it gains nothing (1235 us with eight and with six, 1266 with five), nor do the other kernels.
+template <class PT, class LT>
+constexpr unsigned idle_lds() {
+  return !__is_same(LT, None) ? 160 * 1024 / 5 : sizeof(PT) == 2 ? 160 * 1024 / 6 / 512 * 512 : 0;
+}
+
 template <class PT, class GT, class LT>
 int adam_launch(bool bits8, const AdamArgs<LT>& a, int64_t chunks, hipStream_t stream) {
   const dim3 grid((unsigned)chunks);
+  [[maybe_unused]] constexpr unsigned idle = idle_lds<PT, LT>();
   if (bits8) hipLaunchKernelGGL((adamw8_kernel<PT, GT, LT>), grid, dim3(NT), 0, stream, a);
-  else hipLaunchKernelGGL((adamw_kernel<PT, GT, LT>), grid, dim3(NT), 0, stream, a);
+  else hipLaunchKernelGGL((adamw_kernel<PT, GT, LT>), grid, dim3(NT), idle, stream, a);
   return launched("mi_adamw_update");
 }
 template <class PT, class LT>
