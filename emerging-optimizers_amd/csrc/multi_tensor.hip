@@ -41,7 +41,7 @@ struct AdamTensorCopy : AdamTensor {
   void* low;  // 16-bit copy of the updated weights
 };
 struct AdamScalars {
-  float b1, omb1, b2, omb2, eps, keep, l2, step_size, inv_sqrt_bc2;
+  float b1, omb1, b2, omb2, eps, shrink, l2, step_size, inv_sqrt_bc2;
   // for a step counter or a learning rate on the device: bias corrections and decay are evaluated by the kernel
   int on_device, method;
   double lr, wd, ln_b1, ln_b2, step;
@@ -157,16 +157,16 @@ struct Part {
 // AdamW
 // ---------------------------------------------------------------------------------------------
 struct AdamCoef {
-  float b1, omb1, b2, omb2, eps, keep, l2, step_size, inv_sqrt_bc2, gscale;
+  float b1, omb1, b2, omb2, eps, shrink, l2, step_size, inv_sqrt_bc2, gscale;
 };
 
 enum { DECAY_DECOUPLED = 0, DECAY_INDEPENDENT = 1, DECAY_L2 = 2, DECAY_PALM = 3 };
 
-// Factor of the weight and multiple of the weight that joins the gradient, by decay method.
-__host__ __device__ inline void decay_terms(int method, double wd, double lr, float* keep, float* l2) {
+// Share of the weight that goes, and multiple of the weight that joins the gradient, by decay method.  (The share and not
+// what remains of the weight: 1 - 1e-7 has one digit of the share left in float32.)
+__host__ __device__ inline void decay_terms(int method, double wd, double lr, float* shrink, float* l2) {
   *l2 = method == DECAY_L2 ? (float)wd : 0.0f;
-  const double shrink = method == DECAY_DECOUPLED ? wd * lr : method == DECAY_INDEPENDENT ? wd : method == DECAY_PALM ? wd * lr * lr : 0.0;
-  *keep = (float)(1.0 - shrink);
+  *shrink = (float)(method == DECAY_DECOUPLED ? wd * lr : method == DECAY_INDEPENDENT ? wd : method == DECAY_PALM ? wd * lr * lr : 0.0);
 }
 // lr / (1 - b1^t) and 1 / sqrt(1 - b2^t), in 64 bits: 1 - b^t loses its leading digits for small t and b near 1.
 __host__ __device__ inline void bias_terms(double ln_b1, double ln_b2, double t, double lr, float* step_size, float* inv_sqrt_bc2) {
@@ -175,17 +175,17 @@ __host__ __device__ inline void bias_terms(double ln_b1, double ln_b2, double t,
 }
 
 __device__ __forceinline__ AdamCoef adam_coefficients(const AdamScalars& s, const float* step_dev) {
-  AdamCoef c = {s.b1, s.omb1, s.b2, s.omb2, s.eps, s.keep, s.l2, s.step_size, s.inv_sqrt_bc2, 1.0f};
+  AdamCoef c = {s.b1, s.omb1, s.b2, s.omb2, s.eps, s.shrink, s.l2, s.step_size, s.inv_sqrt_bc2, 1.0f};
   if (s.on_device) {
     const double lr = s.lr_dev ? (double)*s.lr_dev : s.lr;
-    decay_terms(s.method, s.wd, lr, &c.keep, &c.l2);
+    decay_terms(s.method, s.wd, lr, &c.shrink, &c.l2);
     bias_terms(s.ln_b1, s.ln_b2, step_dev ? (double)*step_dev : s.step, lr, &c.step_size, &c.inv_sqrt_bc2);
   }
   if (s.grad_scale) c.gscale = *s.grad_scale;
   return c;
 }
 
-// m <- b1 m + (1 - b1) g,  v <- b2 v + (1 - b2) g^2,  p <- keep p - step_size m / (sqrt(v) inv_sqrt_bc2 + eps)
+// m <- b1 m + (1 - b1) g,  v <- b2 v + (1 - b2) g^2,  p <- p - shrink p - step_size m / (sqrt(v) inv_sqrt_bc2 + eps)
 //
 // FAST: square root and reciprocal of the hardware, each within one unit in the last place, for which a number below the
 // smallest normal one is 0.  The correctly rounded sequences cost about 25 instructions a value: nothing beside 32-bit
@@ -197,7 +197,8 @@ __device__ __forceinline__ void adam_value(float& p, float g, float& m, float& v
   m = fmaf(c.b1, m, c.omb1 * g);
   v = fmaf(c.b2, v, c.omb2 * g * g);
   const float den = fmaf(FAST ? __builtin_amdgcn_sqrtf(v) : sqrtf(v), c.inv_sqrt_bc2, c.eps);
-  p = fmaf(-c.step_size, FAST ? m * __builtin_amdgcn_rcpf(den) : m / den, c.keep * p);
+  if (c.shrink != 0.0f) p = fmaf(-c.shrink, p, p);
+  p = fmaf(-c.step_size, FAST ? m * __builtin_amdgcn_rcpf(den) : m / den, p);
 }
 
 // 32-bit moments.  Each value is read and written once: 28 bytes a value with float32 weights and gradients, 42
@@ -836,7 +837,7 @@ int adam_impl(int64_t count, void* const* param, const void* const* grad, void* 
   s.step = step;
   s.lr_dev = lr_dev;
   s.grad_scale = grad_scale;
-  decay_terms(decay_method, weight_decay, lr, &s.keep, &s.l2);
+  decay_terms(decay_method, weight_decay, lr, &s.shrink, &s.l2);
   if (!step_dev) bias_terms(s.ln_b1, s.ln_b2, step, lr, &s.step_size, &s.inv_sqrt_bc2);
   const int64_t chunk = !bits8 ? ADAM_CHUNK : pb == 2 && gb == 2 ? Adam8Shape<__bf16, __bf16>::CHUNK : Adam8Shape<float, float>::CHUNK;
   const auto entry = [&](int64_t i) { return AdamTensor{param[i], grad[i], exp_avg[i], exp_avg_sq[i], step_dev ? step_dev[i] : nullptr, numel[i]}; };

@@ -247,6 +247,25 @@ def test_the_same_memory_twice_and_half_aligned_moments_are_refused(gpu):
         assert torch.all(t == 1)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("shrink", [1.0, 0.25, 1.5e-7, 3e-7])
+def test_decay_keeps_the_digits_of_its_share(gpu, bits, shrink):
+    """Weights without gradient lose the share ``shrink``, with one rounding of the result, however small the share is
+    beside 1 (and all of themselves at 1)."""
+    gen = torch.Generator().manual_seed(20)
+    p = (torch.randn(5000, generator=gen) * 0.02).to(gpu)
+    start = np64(p)
+    g = torch.zeros_like(p)
+    m, v = torch.zeros_like(p), torch.zeros_like(p)
+    if bits == 8:
+        m, v = (torch.zeros(k.moment_8bit_bytes(5000), dtype=torch.uint8, device=gpu) for _ in range(2))
+    (k.fused_adamw_update if bits == 32 else k.fused_adamw_update_8bit)(
+        [p], [g], [m], [v], step=1, **dict(HYPER, weight_decay=shrink), weight_decay_method="independent"
+    )
+    want = (start - start * float(np.float32(shrink))).astype(np.float32)  # (float64 holds what is rounded to 29 more bits)
+    assert np.array_equal(p.cpu().numpy(), want)
+
+
 def test_extreme_magnitudes_keep_within_float32(gpu):
     """Gradients whose squares underflow leave the update to eps; weights of any size survive."""
     for scale in (1e-30, 1e-20, 1e-10, 1e3, 1e15):
