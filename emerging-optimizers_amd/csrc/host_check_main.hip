@@ -241,15 +241,15 @@ void list_case(const std::vector<int64_t>& sizes, bool quick, int places = 0) {
   const auto bytes_of = [](int dtype) { return dtype == MI_DTYPE_F32 ? 4 : 2; };
   const auto consts = [](const std::vector<void*>& p) { return const_cast<const void* const*>(p.data()); };
   char what[100];
-  for (int bits : {32, 8})
+  for (int bits : {32, 8, 8 | MI_DITHERED})
     for (int param = 0; param < 3; ++param)
       for (int grad = 0; grad < 3; ++grad)
         for (int low = -1; low < 3; ++low) {
           if (low == 0 || (low > 0 && param != 0) || (quick && (param == 2 || grad == 2 || low == 2))) continue;
           std::snprintf(what, sizeof what, "adamw %lld tensors from %lld, bits=%d types=%d %d %d", (long long)count, (long long)sizes[0], bits, param, grad, low);
           begin(what);
-          const auto p = lists(bytes_of(param), "param"), g = lists(bytes_of(grad), "grad"), m = lists(bits == 8 ? 0 : 4, "exp_avg"),
-                     v = lists(bits == 8 ? 0 : 4, "exp_avg_sq"), l = lists(2, "copy");
+          const auto p = lists(bytes_of(param), "param"), g = lists(bytes_of(grad), "grad"), m = lists(bits == 32 ? 4 : 0, "exp_avg"),
+                     v = lists(bits == 32 ? 4 : 0, "exp_avg_sq"), l = lists(2, "copy");
           const int rc = mi_adamw_update(count, p.data(), consts(g), m.data(), v.data(), low > 0 ? l.data() : nullptr, nullptr, sizes.data(), param, grad, low, bits, 1, 1e-3,
                                          nullptr, 0.9, 0.95, 1e-8, 0.1, 0, nullptr, nullptr);
           const int half = low > 0 ? low : param;

@@ -265,11 +265,22 @@ __global__ __launch_bounds__(NT) void adamw_kernel(AdamArgs<LT> a) {
 //   first moment    m = +- s (k / 127)^2   code +-k, k = round(127 sqrt(|m| / s))
 //   second moment   v =    s (k / 255)^4   code   k, k = round(255 (v / s)^(1/4)), at least 1 for v > 0
 // Roots space the codes finer towards 0, evenly in relative terms over a range of 1.6e4 in m and 6e4 in sqrt(v); a
-// second moment over 0 never becomes 0, so no update divides by eps alone.  The rounding is to nearest: with stochastic
-// rounding the noise accumulates over 1 / (1 - beta2) steps and updates end up further from the 32-bit ones (simulated
-// with gradients whose scales spread as exp(N(0, 0.5)), beta2 = 0.95 / 0.999: 2.3 / 4.9 % of the update to nearest, 3.3 /
-// 6.8 % stochastic; linear codes of m and sqrt(v) 3.2 / 5.7 %, e4m3 8.8 / 17 %, and both of these let small second moments
-// of a wide block become 0).
+// second moment over 0 never becomes 0, so no update divides by eps alone (linear codes of m and sqrt(v) and e4m3 let small
+// second moments of a wide block become 0).
+//
+// To nearest is right for one conversion and wrong for a run of steps: a factor b changes code k of m by k (1 - b^(1/2))
+// and of v by k (1 - b^(1/4)), and a code that a step changes by less than half never moves beside a scale that stays (at
+// beta1 = 0.9 the codes up to 9, at beta2 = 0.999 all of v's).  So a run of steps takes DITHERED codes floor(y + u), with
+// y = 127 sqrt(|m| / s) or 255 (v / s)^(1/4) and
+//   u = fraction of (t c + i a)   for step t and place i of the tensor, c and a irrational, others for v than for m.
+// For each place u rotates through its interval evenly, so a change of 0.01 of a code moves it every 100 steps, and the
+// errors of consecutive steps cancel instead of adding up as independent random numbers' do.  Two rules beside it: codes of
+// v below 6 round up (a root of v held at a fraction of itself blows the update up), and the first four steps go to nearest
+// (step t of a moving average changes a code by about 1 / (2 t) of itself, so nothing stands still yet).
+// Simulated update error against 32-bit moments, gradients' scales spread as exp(N(0, sigma)), beta2 = 0.95 / 0.999:
+//   sigma 0.5: nearest 2.3 / 5.6 %, independent random numbers 3.3 / 6.9 %, rotating 2.5 / 5.8 %
+//   sigma 1.5: nearest 11 / 16 %, rotating 12 / 16 %;   sigma 2.5: nearest 84 / 94 %, rotating 40 / 42 %
+//   half of each block's gradients fall to a tenth, beta2 = 0.999: sqrt(v) 4.6 times too large to nearest, 1.0 rotating.
 // A block whose largest magnitude is below the smallest normal number is stored as 0, one that holds a value that is not
 // finite as NaN.  Codes of places behind the last value are 0.
 // ---------------------------------------------------------------------------------------------
@@ -329,6 +340,46 @@ __device__ __forceinline__ Codes<V> encode(Floats<V> x, float s) {
     codes[i / 4] = __builtin_amdgcn_perm(k[i + 1], k[i], 0x0c0c0400u) | __builtin_amdgcn_perm(k[i + 3], k[i + 2], 0x04000c0cu);
   return codes;
 }
+
+// Dithered codes: bits of u as fractions of 2^32, at the lane's first place and from one place to the next, and the root of
+// v / s below which codes round up.
+struct Dither {
+  uint32_t m, v, m_place, v_place;
+  float up;
+};
+constexpr uint32_t DITHER_M_STEP = 0x9E3779B9u;                                      // golden ratio
+constexpr uint32_t DITHER_M_PLACE = 0x6A09E667u, DITHER_V_STEP = 0x6A09E667u;        // sqrt(2)
+constexpr uint32_t DITHER_V_PLACE = 0xBB67AE85u;                                     // sqrt(3)
+constexpr double DITHER_AFTER = 4.0;                                                 // steps to nearest
+__device__ __forceinline__ Dither dither(const AdamScalars& s, const float* step_dev, uint32_t place) {
+  const double t = step_dev ? (double)*step_dev : s.step;
+  if (!(t > DITHER_AFTER)) return {0x80000000u, 0x80000000u, 0u, 0u, 0.0f};  // u = 1/2: to nearest
+  const uint32_t n = (uint32_t)(uint64_t)t;
+  return {n * DITHER_M_STEP + place * DITHER_M_PLACE, n * DITHER_V_STEP + place * DITHER_V_PLACE, DITHER_M_PLACE, DITHER_V_PLACE, 6.0f / 255};
+}
+template <int V, bool SIGNED>
+__device__ __forceinline__ Codes<V> encode_dithered(Floats<V> x, float s, const Dither& d) {
+  float inv = s > 0.0f ? __builtin_amdgcn_rcpf(s) : 0.0f;
+  if (__builtin_expect(s > 0x1p125f, 0)) inv = 1.0f / s;
+  uint32_t k[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float root = __builtin_amdgcn_sqrtf(fabsf(x[i]) * inv);
+    if constexpr (!SIGNED) root = __builtin_amdgcn_sqrtf(root);
+    const uint32_t bits = SIGNED ? d.m + i * d.m_place : d.v + i * d.v_place;
+    float one_u = __uint_as_float(0x3f800000u | bits >> 9);                     // 1 + u
+    if constexpr (!SIGNED) one_u = root < d.up ? 2.0f - 0x1p-8f : one_u;        // (1/256: the roots' own error is no step up)
+    // at most the largest code, whatever the roots' last place is
+    const uint32_t n = (uint32_t)fminf(fmaf(root, SIGNED ? 127.0f : 255.0f, one_u) - 1.0f, SIGNED ? 127.5f : 255.5f);
+    k[i] = SIGNED ? (x[i] < 0.0f ? 0u - n : n) : max(n, x[i] > 0.0f && s > 0.0f ? 1u : 0u);
+  }
+  Codes<V> codes;
+#pragma unroll
+  for (int i = 0; i < V; i += 4)
+    codes[i / 4] = __builtin_amdgcn_perm(k[i + 1], k[i], 0x0c0c0400u) | __builtin_amdgcn_perm(k[i + 3], k[i + 2], 0x04000c0cu);
+  return codes;
+}
+
 template <int V, bool SIGNED>
 __device__ __forceinline__ Floats<V> decode(Codes<V> codes, float s) {
   Floats<V> x;
@@ -366,7 +417,7 @@ struct Adam8Shape {
   static constexpr int V = sizeof(PT) == 2 && sizeof(GT) == 2 ? 8 : 4, CHUNK = NT * V;
 };
 
-template <class PT, class GT, class LT>
+template <class PT, class GT, class LT, bool DITHERED>
 __global__ __launch_bounds__(NT) void adamw8_kernel(AdamArgs<LT> a) {
   typedef Adam8Shape<PT, GT> S;
   constexpr int V = S::V;
@@ -411,8 +462,14 @@ __global__ __launch_bounds__(NT) void adamw8_kernel(AdamArgs<LT> a) {
       if (i >= k) mm[i] = vv[i] = 0.0f;
   }
   const float sm = block_scale<V>(mm), sv = block_scale<V>(vv);
-  store_codes<V>(mc + e, encode<V, true>(mm, sm));
-  store_codes<V>(vc + e, encode<V, false>(vv, sv));
+  if constexpr (DITHERED) {
+    const Dither d = dither(a.s, t.step, (uint32_t)(base + e));
+    store_codes<V>(mc + e, encode_dithered<V, true>(mm, sm, d));
+    store_codes<V>(vc + e, encode_dithered<V, false>(vv, sv, d));
+  } else {
+    store_codes<V>(mc + e, encode<V, true>(mm, sm));
+    store_codes<V>(vc + e, encode<V, false>(vv, sv));
+  }
   if (e % BLOCK8 == 0) {
     ms[b] = sm;
     vs[b] = sv;
@@ -771,20 +828,21 @@ constexpr unsigned idle_lds() {
 }
 
 template <class PT, class GT, class LT>
-int adam_launch(bool bits8, const AdamArgs<LT>& a, int64_t chunks, hipStream_t stream) {
+int adam_launch(int bits, const AdamArgs<LT>& a, int64_t chunks, hipStream_t stream) {
   const dim3 grid((unsigned)chunks);
   [[maybe_unused]] constexpr unsigned idle = idle_lds<PT, LT>();
-  if (bits8) hipLaunchKernelGGL((adamw8_kernel<PT, GT, LT>), grid, dim3(NT), 0, stream, a);
+  if (bits == (8 | MI_DITHERED)) hipLaunchKernelGGL((adamw8_kernel<PT, GT, LT, true>), grid, dim3(NT), 0, stream, a);
+  else if (bits == 8) hipLaunchKernelGGL((adamw8_kernel<PT, GT, LT, false>), grid, dim3(NT), 0, stream, a);
   else hipLaunchKernelGGL((adamw_kernel<PT, GT, LT>), grid, dim3(NT), idle, stream, a);
   return launched("mi_adamw_update");
 }
 template <class PT, class LT>
-int adam_launch_grad(int grad_dtype, bool bits8, const AdamArgs<LT>& a, int64_t chunks, hipStream_t stream) {
-  if (grad_dtype == MI_DTYPE_F32) return adam_launch<PT, float, LT>(bits8, a, chunks, stream);
+int adam_launch_grad(int grad_dtype, int bits, const AdamArgs<LT>& a, int64_t chunks, hipStream_t stream) {
+  if (grad_dtype == MI_DTYPE_F32) return adam_launch<PT, float, LT>(bits, a, chunks, stream);
   if constexpr (!__is_same(PT, _Float16) && !__is_same(LT, _Float16))
-    if (grad_dtype == MI_DTYPE_BF16) return adam_launch<PT, __bf16, LT>(bits8, a, chunks, stream);
+    if (grad_dtype == MI_DTYPE_BF16) return adam_launch<PT, __bf16, LT>(bits, a, chunks, stream);
   if constexpr (!__is_same(PT, __bf16) && !__is_same(LT, __bf16))
-    if (grad_dtype == MI_DTYPE_F16) return adam_launch<PT, _Float16, LT>(bits8, a, chunks, stream);
+    if (grad_dtype == MI_DTYPE_F16) return adam_launch<PT, _Float16, LT>(bits, a, chunks, stream);
   return fail(MI_ERR_BAD_ARG, "mi_adamw_update: bfloat16 and float16 do not go together");
 }
 
@@ -800,13 +858,13 @@ int adam_impl(int64_t count, void* const* param, const void* const* grad, void* 
   const int mixed = model_param ? model_dtype : param_dtype;
   if (mixed != MI_DTYPE_F32 && grad_dtype != MI_DTYPE_F32 && grad_dtype != mixed)
     return fail(MI_ERR_BAD_ARG, "%s: bfloat16 and float16 do not go together", who);
-  if (moment_bits != 32 && moment_bits != 8) return fail(MI_ERR_BAD_ARG, "%s: moments have 32 or 8 bits, got %d", who, moment_bits);
+  if (moment_bits != 32 && moment_bits != 8 && moment_bits != (8 | MI_DITHERED)) return fail(MI_ERR_BAD_ARG, "%s: moments have 32 or 8 bits, got %d", who, moment_bits);
   // (comparisons that NaN fails)
   if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0)) return fail(MI_ERR_BAD_ARG, "%s: betas must be in [0, 1)", who);
   if (!(eps >= 0.0)) return fail(MI_ERR_BAD_ARG, "%s: eps must not be negative", who);
   if (!step_dev && !(step >= 1.0)) return fail(MI_ERR_BAD_ARG, "%s: step must be at least 1", who);
   if (decay_method < DECAY_DECOUPLED || decay_method > DECAY_PALM) return fail(MI_ERR_BAD_ARG, "%s: unknown weight decay method %d", who, decay_method);
-  const bool bits8 = moment_bits == 8;
+  const bool bits8 = moment_bits != 32;
   const int pb = element_bytes(param_dtype), gb = element_bytes(grad_dtype);
   {
     Spans spans;
@@ -867,18 +925,18 @@ int adam_impl(int64_t count, void* const* param, const void* const* grad, void* 
     };
     if (model_dtype == MI_DTYPE_BF16) {
       AdamArgs<__bf16> a;
-      return run(&a, [&](const auto& x, int64_t chunks) { return adam_launch_grad<float, __bf16>(grad_dtype, bits8, x, chunks, stream); });
+      return run(&a, [&](const auto& x, int64_t chunks) { return adam_launch_grad<float, __bf16>(grad_dtype, moment_bits, x, chunks, stream); });
     }
     AdamArgs<_Float16> a;
-    return run(&a, [&](const auto& x, int64_t chunks) { return adam_launch_grad<float, _Float16>(grad_dtype, bits8, x, chunks, stream); });
+    return run(&a, [&](const auto& x, int64_t chunks) { return adam_launch_grad<float, _Float16>(grad_dtype, moment_bits, x, chunks, stream); });
   }
   AdamArgs<None> a;
   a.s = s;
   return for_each_list(count, numel, chunk, a.list, entry, before, [&](const auto& l, int64_t chunks) -> int {
     state_footprints(l, chunks);
-    if (param_dtype == MI_DTYPE_F32) return adam_launch_grad<float, None>(grad_dtype, bits8, a, chunks, stream);
-    if (param_dtype == MI_DTYPE_BF16) return adam_launch_grad<__bf16, None>(grad_dtype, bits8, a, chunks, stream);
-    return adam_launch_grad<_Float16, None>(grad_dtype, bits8, a, chunks, stream);
+    if (param_dtype == MI_DTYPE_F32) return adam_launch_grad<float, None>(grad_dtype, moment_bits, a, chunks, stream);
+    if (param_dtype == MI_DTYPE_BF16) return adam_launch_grad<__bf16, None>(grad_dtype, moment_bits, a, chunks, stream);
+    return adam_launch_grad<_Float16, None>(grad_dtype, moment_bits, a, chunks, stream);
   });
 }
 

@@ -222,7 +222,7 @@ PyObject* guarded(Body body) {
 
 constexpr int ANY_TYPE = 7, F32_ONLY = 1, HALF_TYPES = 6;
 
-// adamw_update(who, bits, params, grads, exp_avgs, exp_avg_sqs, model_params | None, step | steps, lr, beta1, beta2,
+// adamw_update(who, bits (mi_adamw_update's moment_bits), params, grads, exp_avgs, exp_avg_sqs, model_params | None, step | steps, lr, beta1, beta2,
 //              eps, weight_decay, method, grad_scale | None) -> return code
 PyObject* adamw_update(PyObject*, PyObject* args) {
   const char* who;
@@ -238,7 +238,7 @@ PyObject* adamw_update(PyObject*, PyObject* args) {
     const int p_type = params.dtype(ANY_TYPE), g_type = grads.dtype(ANY_TYPE);
     grads.like(params);
     for (const List* l : {&ms, &vs}) {
-      if (bits == 8) {
+      if (bits != 32) {
         l->packed(params);
       } else {
         l->dtype(F32_ONLY);

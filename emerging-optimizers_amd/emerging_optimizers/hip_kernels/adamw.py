@@ -12,9 +12,11 @@ from .. import _hip
 __all__ = ["fused_adamw_update", "fused_adamw_update_8bit", "moment_8bit_bytes", "pack_moments_8bit", "unpack_moments_8bit"]
 
 MomentT = Literal["exp_avg", "exp_avg_sq"]
+RoundingT = Literal["nearest", "dithered"]
 
 _DECAY_METHODS = {"decoupled": 0, "independent": 1, "l2": 2, "palm": 3}
 _MOMENTS = {"exp_avg": 0, "exp_avg_sq": 1}
+_ROUNDING_BITS = {"nearest": 8, "dithered": 8 | 256}
 
 
 def moment_8bit_bytes(numel: int) -> int:
@@ -90,13 +92,23 @@ def fused_adamw_update_8bit(
     weight_decay_method: str = "decoupled",
     grad_scale: Optional[torch.Tensor] = None,
     model_params: Optional[Sequence[torch.Tensor]] = None,
+    rounding: RoundingT = "nearest",
 ) -> None:
     """:func:`fused_adamw_update` with moments in their 8-bit form: ``exp_avgs`` and ``exp_avg_sqs`` are uint8 tensors
     of :func:`moment_8bit_bytes` bytes each, 16-byte aligned (zeros stand for zero moments; see
     :func:`pack_moments_8bit`).  The update uses the new moments before they are rounded to 8 bits.
+
+    ``rounding`` is how the new moments become codes.  "nearest" is the definition of :func:`pack_moments_8bit`, for single
+    updates.  Over a run of steps it stops a moving average whose step is less than half the distance between two codes: with
+    ``beta2=0.999`` a second moment whose gradients shrink never follows them while the largest one of its block stays.
+    "dithered" is for training loops: from the fifth step on the code is the next one below or above, by an offset that rotates
+    with ``step`` (see ``mi_adamw_update``), so moments follow on average; consecutive calls need consecutive ``step``.
     """
+    bits = _ROUNDING_BITS.get(rounding)
+    if bits is None:
+        raise ValueError(f'fused_adamw_update_8bit: rounding must be "nearest" or "dithered", got {rounding!r}')
     rc = _hip.lists().adamw_update(
-        "fused_adamw_update_8bit", 8, params, grads, exp_avgs, exp_avg_sqs, model_params, step, lr, beta1, beta2, eps, weight_decay,
+        "fused_adamw_update_8bit", bits, params, grads, exp_avgs, exp_avg_sqs, model_params, step, lr, beta1, beta2, eps, weight_decay,
         _decay_code(weight_decay_method), grad_scale,
     )  # fmt: skip
     _hip.check(rc)

@@ -228,6 +228,8 @@ int mi_muon_update_bf16(float* param, const float* grad, float* momentum, int64_
 #define MI_DTYPE_BF16 1
 #define MI_DTYPE_F16 2
 
+#define MI_DITHERED 256 /* with moment_bits 8 of mi_adamw_update */
+
 /* Weight-decay methods (mixin.py:35-56 of the reference): what multiplies the weight, or joins the gradient. */
 #define MI_DECAY_DECOUPLED 0   /* param *= 1 - weight_decay * lr    */
 #define MI_DECAY_INDEPENDENT 1 /* param *= 1 - weight_decay         */
@@ -243,7 +245,14 @@ int mi_muon_update_bf16(float* param, const float* grad, float* momentum, int64_
  * param: weights of record, float32, bfloat16 or float16 (param_dtype).  model_param: NULL, or 16-bit copies
  * (model_dtype) of float32 weights, written only.  grad: float32, or the 16-bit type that the weights or their copies
  * have (either one for float32 weights without copies).  exp_avg, exp_avg_sq: the moments m and v, updated in place;
- * moment_bits == 32: float32 values; moment_bits == 8: the 8-bit form described at mi_moments_8bit_pack.
+ * moment_bits == 32: float32 values; moment_bits == 8: the 8-bit form described at mi_moments_8bit_pack;
+ * moment_bits == (8 | MI_DITHERED): the same form, with codes that are dithered instead of rounded to nearest from the
+ * fifth step on.  To nearest is the definition of one conversion.  Over a run of steps it stops a moving average whose step is
+ * less than half the distance between two codes (with beta2 = 0.999 every one), so a training loop takes MI_DITHERED:
+ *   |k| = floor(y + u), y = 127 sqrt(|m| / s) or 255 (v / s)^(1/4), at most 127 or 255,
+ *   u = ((t * c + i * a) mod 2^32 >> 9) / 2^23 for place i of the tensor (in memory order) and the whole part of t,
+ *   c, a = 0x9E3779B9, 0x6A09E667 for m and 0x6A09E667, 0xBB67AE85 for v; u = 255/256 for y < 6 in v; u = 1/2 for t <= 4.
+ * Consecutive steps have to have consecutive t; the same call gives the same codes.
  * (With 8-bit moments a second moment below 2^-126 counts as 0, in the update too.)
  * t = step (>= 1), or, where step_dev is not NULL, *step_dev[i] for tensor i (float32 on the device).
  * lr_dev: NULL, or a float32 on the device that replaces lr.  grad_scale: NULL (1), or a float32 on the device.
