@@ -322,7 +322,7 @@ template <int V, bool SIGNED>
 __device__ __forceinline__ Codes<V> encode(Floats<V> x, float s) {
   float inv = s > 0.0f ? __builtin_amdgcn_rcpf(s) : 0.0f;  // (neither for 0 nor for NaN)
   if (__builtin_expect(s > 0x1p125f, 0)) inv = 1.0f / s;   // below the smallest normal number, which v_rcp_f32 makes 0
-  const uint32_t least = s > 0.0f ? 1u : 0u;
+  const int least = s > 0.0f ? 1 : 0;
   uint32_t k[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -331,7 +331,8 @@ __device__ __forceinline__ Codes<V> encode(Floats<V> x, float s) {
       k[i] = __float_as_uint(fmaf(copysignf(root, x[i]), 127.0f, 12582912.0f));
     } else {
       k[i] = __float_as_uint(fmaf(__builtin_amdgcn_sqrtf(root), 255.0f, 12582912.0f));
-      k[i] = max(k[i], 0x4B400000u | min(__float_as_uint(x[i]), least));  // 1 at least for a value over 0
+      // 1 at least for a value over 0 (as integers -0.0 and negative values are below 0)
+      k[i] = max(k[i], 0x4B400000u | (uint32_t)max(min(__float_as_int(x[i]), least), 0));
     }
   }
   Codes<V> codes;

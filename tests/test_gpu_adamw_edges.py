@@ -1,0 +1,32 @@
+"""Edges of the multi-tensor operators on the GPU: signed zeros and negative values, full argument blocks, memory around
+tensors of 16 bits, odd places."""
+
+import numpy as np
+import pytest
+import torch
+
+import _adamw_oracle as O
+from emerging_optimizers import hip_kernels as k
+from emerging_optimizers.scalar_optimizers.adamw import _pack_torch
+from test_gpu_adamw import BF16, F16, F32, HYPER, check_update, moments, np64, packed_like, snapshot, values
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_negative_zeros_and_negative_values_in_second_moments(gpu, dtype):
+    """Only a value over 0 gets the smallest code at least; -0.0 and a negative value that rounds to 0 get 0."""
+    x = torch.zeros(200, dtype=dtype)
+    x[0], x[64], x[128] = 2.0, 3.0, 1.0
+    x[1:64:2] = -0.0
+    x[65:120:3] = -1e-7 if dtype == F16 else -1e-12  # below (0.5 / 255)^4 of 3, the smallest that rounds to code 1, is 4e-11
+    x[66:120:3] = 1e-7 if dtype == F16 else 1e-12
+    x[130] = -0.5
+    packed = packed_like([x.to(gpu)], "exp_avg_sq")[0].cpu()
+    codes = packed[:200].to(torch.int64)
+    assert not codes[1:64].any()
+    if dtype != F16:
+        assert not codes[65:120:3].any()
+    assert torch.all(codes[66:120:3] >= 1)
+    O.check_packed(packed.numpy(), np64(x), np.zeros(200), "exp_avg_sq")
+    assert torch.equal(packed, _pack_torch(x.float(), "exp_avg_sq"))
