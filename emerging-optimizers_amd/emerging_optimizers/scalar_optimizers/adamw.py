@@ -274,7 +274,11 @@ class AdamW(WeightDecayMixin, Optimizer):
     @torch.no_grad()
     def load_state_dict(self, state_dict: dict) -> None:
         """Loads a checkpoint of this class or of ``torch.optim.AdamW``.  Moments come in either width and are held in
-        the one of this optimizer; a missing float32 copy of a 16-bit parameter is made from the parameter."""
+        the one of this optimizer; a missing float32 copy of a 16-bit parameter is made from the parameter.  Refuses what
+        this class would continue another way: ``maximize``, ``amsgrad``, and ``torch.optim.Adam``'s coupled weight decay
+        (unless ``weight_decay_method`` is "l2", which is that)."""
+        for group in state_dict["param_groups"]:
+            self._check_loaded_group(group)
         super().load_state_dict(state_dict)
         saved = state_dict["state"]
         for group, saved_group in zip(self.param_groups, state_dict["param_groups"]):
@@ -291,6 +295,13 @@ class AdamW(WeightDecayMixin, Optimizer):
                     state["master"] = torch.empty_like(p, dtype=torch.float32).copy_(saved[index].get("master", p.detach()))
                 else:
                     state.pop("master", None)
+
+    def _check_loaded_group(self, group: dict) -> None:
+        for option in ("maximize", "amsgrad"):
+            if group.get(option):
+                raise ValueError(f"AdamW cannot continue a checkpoint with {option}=True")
+        if not group.get("decoupled_weight_decay", True) and group["weight_decay"] != 0 and self.weight_decay_method != "l2":
+            raise ValueError(f'the checkpoint\'s weight decay is not decoupled, which is weight_decay_method="l2" and not "{self.weight_decay_method}"')
 
     def _loaded_moment(self, value: torch.Tensor, p: torch.Tensor, which: str) -> torch.Tensor:
         """A moment of a checkpoint in the width and the memory order that this optimizer holds it in."""

@@ -1,0 +1,55 @@
+"""Checkpoints and copies of AdamW: what cannot be continued is refused before anything changes, what can be is whole."""
+
+import copy
+import pickle
+
+import pytest
+import torch
+
+from emerging_optimizers.scalar_optimizers import AdamW
+
+
+def stepped(cls=AdamW, shape=(6,), dtype=torch.float32, **kwargs):
+    """An optimizer of one parameter after one step, and the parameter."""
+    p = torch.nn.Parameter(torch.linspace(-1, 1, 6).reshape(shape).to(dtype))
+    opt = cls([p], **kwargs)
+    p.grad = torch.linspace(0.5, 1.5, 6).reshape(shape).to(dtype)
+    opt.step()
+    return opt, p
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize(
+    "cls, options, text",
+    [
+        (torch.optim.AdamW, dict(maximize=True), "maximize"),
+        (torch.optim.AdamW, dict(amsgrad=True), "amsgrad"),
+        (torch.optim.Adam, dict(weight_decay=0.1), "decoupled"),
+    ],
+)
+def test_checkpoints_of_another_rule_are_refused(cls, options, text, bits):
+    """Gradients followed upwards, the running maximum of second moments, decay that goes through the moments: a step of
+    this class would go another way than the run that is continued."""
+    theirs, _ = stepped(cls, lr=0.1, **options)
+    mine, p = stepped(lr=0.3, moment_bits=bits)
+    before = copy.deepcopy(mine.state_dict())
+    with pytest.raises(ValueError, match=text):
+        mine.load_state_dict(theirs.state_dict())
+    after = mine.state_dict()
+    assert after["param_groups"] == before["param_groups"]
+    assert all(torch.equal(torch.as_tensor(a), torch.as_tensor(b)) for a, b in zip(after["state"][0].values(), before["state"][0].values()))
+
+
+def test_checkpoints_of_the_same_rule_load():
+    for cls, options in ((torch.optim.AdamW, dict(weight_decay=0.1)), (torch.optim.Adam, dict(weight_decay=0.0))):
+        theirs, p = stepped(cls, lr=0.1, **options)
+        q = torch.nn.Parameter(p.detach().clone())
+        mine = AdamW([q], lr=0.3)
+        mine.load_state_dict(theirs.state_dict())
+        q.grad = p.grad
+        for opt in (theirs, mine):
+            opt.step()
+        # each side rounds its moments, the quotient and the weight: about 10 roundings of an update of 0.1
+        torch.testing.assert_close(q, p, rtol=2 * 2.0**-24, atol=10 * 0.1 * 2.0**-24)
+    theirs, p = stepped(torch.optim.Adam, lr=0.1, weight_decay=0.1)
+    AdamW([p], weight_decay_method="l2").load_state_dict(theirs.state_dict())
