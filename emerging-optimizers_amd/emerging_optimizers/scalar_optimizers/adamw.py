@@ -276,10 +276,19 @@ class AdamW(WeightDecayMixin, Optimizer):
         """Loads a checkpoint of this class or of ``torch.optim.AdamW``.  Moments come in either width and are held in
         the one of this optimizer; a missing float32 copy of a 16-bit parameter is made from the parameter.  Refuses what
         this class would continue another way: ``maximize``, ``amsgrad``, and ``torch.optim.Adam``'s coupled weight decay
-        (unless ``weight_decay_method`` is "l2", which is that)."""
+        (unless ``weight_decay_method`` is "l2", which is that).  A refused load changes nothing."""
         for group in state_dict["param_groups"]:
             self._check_loaded_group(group)
-        super().load_state_dict(state_dict)
+        before = self.state, self.param_groups
+        try:
+            super().load_state_dict(state_dict)  # (puts new dictionaries in the place of both)
+            self._take_states(state_dict)
+        except BaseException:
+            self.state, self.param_groups = before
+            raise
+
+    def _take_states(self, state_dict: dict) -> None:
+        """Every loaded state in the widths and types of this optimizer, from the checkpoint itself."""
         saved = state_dict["state"]
         for group, saved_group in zip(self.param_groups, state_dict["param_groups"]):
             for p, index in zip(group["params"], saved_group["params"]):

@@ -53,3 +53,45 @@ def test_checkpoints_of_the_same_rule_load():
         torch.testing.assert_close(q, p, rtol=2 * 2.0**-24, atol=10 * 0.1 * 2.0**-24)
     theirs, p = stepped(torch.optim.Adam, lr=0.1, weight_decay=0.1)
     AdamW([p], weight_decay_method="l2").load_state_dict(theirs.state_dict())
+
+
+def same(a, b):
+    """Whether two state dictionaries hold the same."""
+    if isinstance(a, dict):
+        return isinstance(b, dict) and a.keys() == b.keys() and all(same(a[key], b[key]) for key in a)
+    if isinstance(a, (list, tuple)):
+        return len(a) == len(b) and all(map(same, a, b))
+    if isinstance(a, torch.Tensor):
+        return isinstance(b, torch.Tensor) and a.dtype == b.dtype and torch.equal(a, b)
+    return a == b
+
+
+@pytest.mark.parametrize("how, bits", [(how, bits) for how in ("shape", "packed size", "missing moment") for bits in (32, 8)] + [("transposed parameter", 8)])
+def test_a_refused_load_changes_nothing(how, bits):
+    """Whatever is wrong with the second of two parameters' states, the optimizer goes on as if nothing had been loaded."""
+
+    def make(lr):
+        ps = [torch.nn.Parameter(torch.linspace(-1, 1, 70).bfloat16()), torch.nn.Parameter(torch.linspace(0, 1, 12).view(3, 4).bfloat16())]
+        opt = AdamW(ps, lr=lr, moment_bits=bits)
+        for p in ps:
+            p.grad = torch.ones_like(p)
+        opt.step()
+        return opt, ps
+
+    saved, (mine, ps) = make(0.5)[0].state_dict(), make(0.1)
+    bad = saved["state"][1]
+    if how == "shape":
+        bad["exp_avg_sq"] = torch.zeros(4, 3)
+    elif how == "packed size":
+        bad["exp_avg"] = torch.zeros(136, dtype=torch.uint8)
+    elif how == "missing moment":
+        del bad["exp_avg"]
+    else:
+        ps[1].data = ps[1].data.t().contiguous().t()
+    before = copy.deepcopy(mine.state_dict())
+    with pytest.raises((ValueError, KeyError)):
+        mine.load_state_dict(saved)
+    assert same(mine.state_dict(), before)
+    if how != "transposed parameter":
+        mine.step()
+        assert mine.state[ps[0]]["step"] == 2
