@@ -277,15 +277,24 @@ class AdamW(WeightDecayMixin, Optimizer):
         the one of this optimizer; a missing float32 copy of a 16-bit parameter is made from the parameter.  Refuses what
         this class would continue another way: ``maximize``, ``amsgrad``, and ``torch.optim.Adam``'s coupled weight decay
         (unless ``weight_decay_method`` is "l2", which is that).  A refused load changes nothing."""
-        for group in state_dict["param_groups"]:
-            self._check_loaded_group(group)
         before = self.state, self.param_groups
+        loaded = state_dict
+
+        def last(_, handed_over: dict) -> None:  # sees what the hooks before the load made of the dictionary
+            nonlocal loaded
+            loaded = handed_over
+            for group in loaded["param_groups"]:
+                self._check_loaded_group(group)
+
+        hook = self.register_load_state_dict_pre_hook(last)
         try:
             super().load_state_dict(state_dict)  # (puts new dictionaries in the place of both)
-            self._take_states(state_dict)
+            self._take_states(loaded)
         except BaseException:
             self.state, self.param_groups = before
             raise
+        finally:
+            hook.remove()
 
     def _take_states(self, state_dict: dict) -> None:
         """Every loaded state in the widths and types of this optimizer, from the checkpoint itself."""

@@ -95,3 +95,27 @@ def test_a_refused_load_changes_nothing(how, bits):
     if how != "transposed parameter":
         mine.step()
         assert mine.state[ps[0]]["step"] == 2
+
+
+def test_load_hooks_see_and_change_what_is_loaded():
+    """A hook before the load may hand over another dictionary: its moments are taken, not the caller's."""
+    theirs, p = stepped(lr=0.1)
+    saved = theirs.state_dict()
+    renamed = {"state": {0: {"step": 1, "m": saved["state"][0]["exp_avg"], "v": saved["state"][0]["exp_avg_sq"]}}, "param_groups": saved["param_groups"]}
+
+    def names(opt, loaded):
+        state = {i: {"step": s["step"], "exp_avg": s["m"] * 2, "exp_avg_sq": s["v"]} for i, s in loaded["state"].items()}
+        return {**loaded, "state": state}
+
+    mine = AdamW([p], lr=0.3)
+    handle = mine.register_load_state_dict_pre_hook(names)
+    mine.load_state_dict(renamed)
+    assert torch.equal(mine.state[p]["exp_avg"], 2 * saved["state"][0]["exp_avg"]) and mine.param_groups[0]["lr"] == 0.1
+    handle.remove()
+    mine.load_state_dict(saved)
+    assert torch.equal(mine.state[p]["exp_avg"], saved["state"][0]["exp_avg"])
+    upwards = copy.deepcopy(saved)
+    mine.register_load_state_dict_pre_hook(lambda opt, loaded: {**upwards, "param_groups": [{**upwards["param_groups"][0], "maximize": True}]})
+    with pytest.raises(ValueError, match="maximize"):
+        mine.load_state_dict(saved)
+    assert len(mine._optimizer_load_state_dict_pre_hooks) == 1
