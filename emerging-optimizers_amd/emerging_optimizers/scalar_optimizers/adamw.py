@@ -143,23 +143,24 @@ class AdamW(WeightDecayMixin, Optimizer):
             # their bytes say nothing about an order of the dimensions, so a checkpoint could not be checked against it
             raise ValueError("8-bit moments need contiguous parameters")
 
-    def _init_param(self, p: torch.Tensor, state: dict) -> None:
+    def _init_param(self, p: torch.Tensor) -> dict:
+        """Makes the state of ``p``, whole or not at all."""
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             # the zeros would be part of the graph and every replay would start from them
             raise RuntimeError("AdamW needs a step before the one that is captured, to make its state")
         self._check_param(p)
-        state["step"] = self._first_step(p)
-        state["exp_avg"] = self._moment(p)
-        state["exp_avg_sq"] = self._moment(p)
+        state = {"step": self._first_step(p), "exp_avg": self._moment(p), "exp_avg_sq": self._moment(p)}
         if self.master_weights and p.dtype in (torch.bfloat16, torch.float16):
             state["master"] = p.detach().to(torch.float32)
+        self.state[p] = state
+        return state
 
     @torch.no_grad()
     def _init_group(self, group: dict, skip_non_grad_params: bool = True) -> None:
         """Creates the state of every parameter of ``group`` that does not have one yet."""
         for p in group["params"]:
-            if (p.grad is not None or not skip_non_grad_params) and not self.state[p]:
-                self._init_param(p, self.state[p])
+            if (p.grad is not None or not skip_non_grad_params) and not self.state.get(p):
+                self._init_param(p)
 
     @torch.no_grad()
     def step(self, closure: Optional[Callable[[], float]] = None, *, grad_scale: Optional[torch.Tensor] = None) -> Optional[float]:
@@ -182,9 +183,7 @@ class AdamW(WeightDecayMixin, Optimizer):
                     continue
                 if grad.is_sparse:
                     raise RuntimeError("AdamW does not support sparse gradients")
-                state = self.state[p]
-                if not state:
-                    self._init_param(p, state)
+                state = self.state.get(p) or self._init_param(p)
                 key = (p.dtype, grad.dtype, p.get_device(), "master" in state, None if self.capturable else state["step"])
                 if key != last:
                     last = key

@@ -119,3 +119,15 @@ def test_load_hooks_see_and_change_what_is_loaded():
     with pytest.raises(ValueError, match="maximize"):
         mine.load_state_dict(saved)
     assert len(mine._optimizer_load_state_dict_pre_hooks) == 1
+
+
+def test_a_refused_first_step_leaves_no_state():
+    p = torch.nn.Parameter(torch.ones(4, 1).expand(4, 4))
+    p.grad = torch.ones(4, 4)
+    opt = AdamW([p])
+    for call in (opt.step, lambda: opt._init_group(opt.param_groups[0])):
+        with pytest.raises(ValueError, match="fill their memory"):
+            call()
+        assert p not in opt.state
+    q = torch.nn.Parameter(torch.ones(4, 4))
+    AdamW([q]).load_state_dict(opt.state_dict())
