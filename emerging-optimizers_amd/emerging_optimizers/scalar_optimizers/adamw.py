@@ -125,6 +125,11 @@ class AdamW(WeightDecayMixin, Optimizer):
         self.capturable = bool(capturable)
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
+    def __getstate__(self) -> dict:
+        # the base class copies and pickles options, state and parameter groups only
+        own = ("weight_decay_method", "moment_bits", "master_weights", "capturable")
+        return {**super().__getstate__(), **{name: getattr(self, name) for name in own}}
+
     def _moment(self, p: torch.Tensor) -> torch.Tensor:
         """A zero moment of ``p``."""
         if self.moment_bits == 8:

@@ -131,3 +131,20 @@ def test_a_refused_first_step_leaves_no_state():
         assert p not in opt.state
     q = torch.nn.Parameter(torch.ones(4, 4))
     AdamW([q]).load_state_dict(opt.state_dict())
+
+
+@pytest.mark.parametrize("make", [copy.deepcopy, lambda opt: pickle.loads(pickle.dumps(opt))], ids=["deepcopy", "pickle"])
+@pytest.mark.parametrize(
+    "options", [dict(), dict(moment_bits=8, weight_decay_method="independent"), dict(master_weights=True, weight_decay_method="palm"), dict(capturable=True)]
+)
+def test_copies_go_on_as_the_original(make, options):
+    opt, p = stepped(dtype=torch.bfloat16, lr=0.1, **options)
+    twin = make(opt)
+    q = twin.param_groups[0]["params"][0]
+    assert q is not p and torch.equal(q, p)
+    for _ in range(3):
+        p.grad = torch.linspace(-1, 1, 6).bfloat16()
+        q.grad = p.grad.clone()
+        opt.step()
+        twin.step()
+    assert torch.equal(q, p) and same(opt.state_dict(), twin.state_dict())
