@@ -157,8 +157,9 @@ class AdamW(WeightDecayMixin, Optimizer):
         state = {"step": self._first_step(p), "exp_avg": self._moment(p), "exp_avg_sq": self._moment(p)}
         if self.master_weights and p.dtype in (torch.bfloat16, torch.float16):
             state["master"] = p.detach().to(torch.float32)
-        self.state[p] = state
-        return state
+        held = self.state[p]  # (a dictionary that a caller may hold already)
+        held.update(state)
+        return held
 
     @torch.no_grad()
     def _init_group(self, group: dict, skip_non_grad_params: bool = True) -> None:

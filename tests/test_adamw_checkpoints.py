@@ -131,6 +131,11 @@ def test_a_refused_first_step_leaves_no_state():
         assert p not in opt.state
     q = torch.nn.Parameter(torch.ones(4, 4))
     AdamW([q]).load_state_dict(opt.state_dict())
+    q.grad = torch.ones(4, 4)
+    opt = AdamW([q])
+    held = opt.state[q]
+    opt.step()
+    assert held is opt.state[q] and held["step"] == 1
 
 
 @pytest.mark.parametrize("make", [copy.deepcopy, lambda opt: pickle.loads(pickle.dumps(opt))], ids=["deepcopy", "pickle"])
