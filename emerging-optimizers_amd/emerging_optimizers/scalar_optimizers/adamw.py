@@ -253,20 +253,27 @@ class AdamW(WeightDecayMixin, Optimizer):
 
     def _update_torch(self, p: torch.Tensor, group: dict, grad_scale: Optional[torch.Tensor]) -> None:
         """The update of one parameter as torch statements, in float32 (float64 parameters: in float64)."""
-        state, lr, (beta1, beta2) = self.state[p], float(group["lr"]), group["betas"]
+        state, lr, (beta1, beta2) = self.state[p], group["lr"], group["betas"]
+        # a count and a rate on the device stay there (in 64 bits: 1 - beta**t loses its digits in 32), so the statements can
+        # be captured
+        t = state["step"].double() if self.capturable else state["step"]
+        if isinstance(lr, torch.Tensor):
+            lr = lr.reshape(()).double() if lr.device == p.device else float(lr)
         held = state.get("master", p)
         wide = torch.promote_types(p.dtype, torch.float32)
         w, grad = held.to(wide, copy=True), p.grad.to(wide, copy=True)
         if grad_scale is not None:
             grad.mul_(grad_scale)
-        self._apply_weight_decay_inplace(w, grad, lr, group["weight_decay"])
+        if isinstance(lr, torch.Tensor) and self.weight_decay_method in ("decoupled", "palm"):
+            w.sub_(w * (group["weight_decay"] * (lr if self.weight_decay_method == "decoupled" else lr * lr)))
+        else:
+            self._apply_weight_decay_inplace(w, grad, lr, group["weight_decay"])
         if self.moment_bits == 8:
             m, v = (_unpack_torch(state[k], p.numel(), k).view(w.shape) for k in ("exp_avg", "exp_avg_sq"))
         else:
             m, v = state["exp_avg"], state["exp_avg_sq"]
         m.lerp_(grad, 1 - beta1)
         v.mul_(beta2).addcmul_(grad, grad, value=1 - beta2)
-        t = state["step"]
         den = (v / (1 - beta2**t)).sqrt_().add_(group["eps"])
         w.sub_(lr / (1 - beta1**t) * (m / den))
         if self.moment_bits == 8:

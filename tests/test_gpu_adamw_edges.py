@@ -7,6 +7,7 @@ import torch
 
 import _adamw_oracle as O
 from emerging_optimizers import hip_kernels as k
+from emerging_optimizers.scalar_optimizers import AdamW
 from emerging_optimizers.scalar_optimizers.adamw import _pack_torch
 from test_gpu_adamw import BF16, F16, F32, HYPER, check_update, moments, np64, packed_like, snapshot, values
 
@@ -30,3 +31,33 @@ def test_negative_zeros_and_negative_values_in_second_moments(gpu, dtype):
     assert torch.all(codes[66:120:3] >= 1)
     O.check_packed(packed.numpy(), np64(x), np.zeros(200), "exp_avg_sq")
     assert torch.equal(packed, _pack_torch(x.float(), "exp_avg_sq"))
+
+
+@pytest.mark.parametrize("bits, dtypes", [(32, (torch.float64, torch.float64)), (32, (BF16, F16)), (8, (BF16, F16))], ids=str)
+@pytest.mark.parametrize("method", ["decoupled", "l2"])
+def test_torch_statements_are_captured_with_tensors(gpu, bits, dtypes, method):
+    """Parameters that the kernels do not serve, with a step count and a learning rate on the device: nothing waits for the
+    GPU, and replays equal eager steps."""
+    p_type, g_type = dtypes
+    gen = torch.Generator().manual_seed(52)
+    start = torch.randn(100, generator=gen).to(p_type)
+    ps = [torch.nn.Parameter(start.to(gpu)) for _ in range(2)]
+    opts = [AdamW([p], lr=torch.tensor(0.01, device=gpu), weight_decay=0.1, weight_decay_method=method, moment_bits=bits, capturable=True) for p in ps]
+    for p, opt in zip(ps, opts):
+        p.grad_dtype = None  # (a gradient of another type than its parameter's)
+        p.grad = torch.zeros(100, dtype=g_type, device=gpu)
+        opt.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opts[0].step()
+    for turn in range(6):
+        g = torch.randn(100, generator=gen).to(g_type).to(gpu)
+        for p, opt in zip(ps, opts):
+            p.grad.copy_(g)
+            opt.param_groups[0]["lr"].fill_(0.01 / (turn + 1))
+        graph.replay()
+        opts[1].step()
+        torch.cuda.synchronize()
+        assert torch.equal(*ps) and not torch.equal(ps[0].cpu(), start)
+        assert float(opts[0].state[ps[0]]["step"]) == turn + 2
