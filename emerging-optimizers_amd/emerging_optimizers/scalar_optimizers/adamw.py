@@ -109,21 +109,34 @@ class AdamW(WeightDecayMixin, Optimizer):
         master_weights: bool = False,
         capturable: bool = False,
     ) -> None:
-        if not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0:
-            raise ValueError(f"betas must be in [0, 1), got {betas}")
-        if not eps >= 0.0:
-            raise ValueError(f"eps must not be negative, got {eps}")
         if moment_bits not in (8, 32):
             raise ValueError(f"moment_bits must be 8 or 32, got {moment_bits}")
-        if isinstance(lr, torch.Tensor) and not capturable:
-            raise ValueError("a learning rate in a tensor needs capturable=True")
         if weight_decay_method not in ("decoupled", "independent", "l2", "palm"):
             raise ValueError(f"Invalid weight decay method: {weight_decay_method}")
         self.weight_decay_method = weight_decay_method
         self.moment_bits = moment_bits
         self.master_weights = bool(master_weights)
         self.capturable = bool(capturable)
-        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+        defaults = dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay)
+        self._check_options(defaults)
+        super().__init__(params, defaults)
+
+    def _check_options(self, options: dict) -> None:
+        betas, lr = options["betas"], options["lr"]
+        if not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0:
+            raise ValueError(f"betas must be in [0, 1), got {betas}")
+        if not options["eps"] >= 0.0:
+            raise ValueError(f"eps must not be negative, got {options['eps']}")
+        if isinstance(lr, torch.Tensor) and not self.capturable:
+            raise ValueError("a learning rate in a tensor needs capturable=True")
+        if not lr >= 0.0:
+            raise ValueError(f"the learning rate must not be negative, got {lr}")
+
+    def add_param_group(self, param_group: dict) -> None:
+        """Adds a group, whose own options are checked as the constructor's are."""
+        if isinstance(param_group, dict):
+            self._check_options({**self.defaults, **param_group})
+        super().add_param_group(param_group)
 
     def __getstate__(self) -> dict:
         # the base class copies and pickles options, state and parameter groups only
