@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from emerging_optimizers.scalar_optimizers import AdamW
+from emerging_optimizers.utils import clip_grad_norm_
 
 
 def param():
@@ -40,3 +41,41 @@ def test_good_options_of_groups_are_taken():
         opt.add_param_group([param()])
     with pytest.raises(ValueError, match="learning rate"):
         AdamW([param()], capturable=True, lr=torch.tensor(-0.5))
+
+
+def grads(gen, device="cpu"):
+    ps = [torch.nn.Parameter(torch.zeros(7, 3, device=device)), torch.nn.Parameter(torch.zeros(5, device=device))]
+    for p in ps:
+        p.grad = torch.randn(p.shape, generator=gen).to(device)
+    return ps
+
+
+def test_norm_type_is_an_argument_as_in_torch():
+    gen = torch.Generator().manual_seed(61)
+    ps = grads(gen)
+    raw = [p.grad.clone() for p in ps]
+    want = torch.nn.utils.clip_grad_norm_(ps, 0.5, 2.0)
+    scaled = [p.grad.clone() for p in ps]
+    for norm_type in (2, 2.0):
+        for p, g in zip(ps, raw):
+            p.grad = g.clone()
+        torch.testing.assert_close(clip_grad_norm_(ps, 0.5, norm_type), want, rtol=8 * 2.0**-24, atol=0)
+        for p, g in zip(ps, scaled):
+            torch.testing.assert_close(p.grad, g, rtol=16 * 2.0**-24, atol=0)
+    for norm_type in (1.0, float("inf"), 0):
+        with pytest.raises(ValueError, match="norm_type"):
+            clip_grad_norm_(ps, 0.5, norm_type)
+    with pytest.raises(TypeError):
+        clip_grad_norm_(ps, 0.5, 2.0, True)
+
+
+def test_a_gradient_listed_twice_counts_and_is_scaled_twice():
+    gen = torch.Generator().manual_seed(62)
+    ps = grads(gen)
+    raw = [p.grad.clone() for p in ps]
+    norm = clip_grad_norm_([*ps, ps[0]], 0.5)
+    exact = float((2 * raw[0].double().square().sum() + raw[1].double().square().sum()).sqrt())
+    assert abs(float(norm) - exact) <= 2 * 2.0**-24 * exact
+    factor = 0.5 / (exact + 1e-6)
+    torch.testing.assert_close(ps[0].grad, raw[0] * factor**2, rtol=16 * 2.0**-24, atol=0)
+    torch.testing.assert_close(ps[1].grad, raw[1] * factor, rtol=16 * 2.0**-24, atol=0)

@@ -9,6 +9,7 @@ import _adamw_oracle as O
 from emerging_optimizers import hip_kernels as k
 from emerging_optimizers.scalar_optimizers import AdamW
 from emerging_optimizers.scalar_optimizers.adamw import _pack_torch
+from emerging_optimizers.utils import clip_grad_norm_
 from test_gpu_adamw import BF16, F16, F32, HYPER, check_update, moments, np64, packed_like, snapshot, values
 
 pytestmark = pytest.mark.gpu
@@ -61,3 +62,20 @@ def test_torch_statements_are_captured_with_tensors(gpu, bits, dtypes, method):
         torch.cuda.synchronize()
         assert torch.equal(*ps) and not torch.equal(ps[0].cpu(), start)
         assert float(opts[0].state[ps[0]]["step"]) == turn + 2
+
+
+@pytest.mark.parametrize("error_if_nonfinite", [False, True])
+def test_a_gradient_listed_twice_counts_and_is_scaled_twice(gpu, error_if_nonfinite):
+    """As with torch, whose convention clip_grad_norm_ follows; the kernels write no place twice, so such a list goes through
+    torch statements."""
+    gen = torch.Generator().manual_seed(62)
+    ps = [torch.nn.Parameter(torch.zeros(n, device=gpu)) for n in (700, 5)]
+    for p in ps:
+        p.grad = torch.randn(p.shape, generator=gen).to(gpu)
+    raw = [np64(p.grad) for p in ps]
+    norm = clip_grad_norm_([*ps, ps[0]], 0.5, error_if_nonfinite=error_if_nonfinite)
+    exact = float(np.sqrt(2 * (raw[0] ** 2).sum() + (raw[1] ** 2).sum()))
+    assert abs(float(norm) - exact) <= 2 * O.U * exact
+    factor = 0.5 / (exact + 1e-6)
+    for p, g, f in zip(ps, raw, (factor**2, factor)):
+        O.assert_within(np64(p.grad), g * f, 16 * O.U * abs(g * f), "clipped")
