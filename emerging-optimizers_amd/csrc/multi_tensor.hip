@@ -819,10 +819,14 @@ int check_numel(const char* who, int64_t count, const int64_t* numel) {
 }
 
 // LDS that a workgroup of the step with 32-bit moments holds without using it, so that fewer than eight of them share a CU:
-// with seven or eight streams of two element sizes in flight, the memory does better with fewer rows open at once.  With
-// 16-bit copies five workgroups (436M values in 19 tensors: 2280 us a clipped step with eight, 2251 with seven, 2216 with
-// six, 2197 with five and four), with 16-bit weights alone six (268M: 970 us with eight, 936 with six, 942 with five); with
-// float32 throughout it gains nothing (1235 us with eight and with six, 1266 with five), nor do the other kernels.
+// the memory does better with fewer rows open at once where 16-bit weights or copies are written beside 32-bit moments.
+// Chosen by what is written, both sides measured (2^28 values in 16 tensors):
+//   16-bit copies, five workgroups: bfloat16 gradients 1255 -> 1232 us, float32 ones 1450 -> 1418
+//     (436M values in 19 tensors, clipped: 2280 us with eight, 2251 seven, 2216 six, 2197 five and four)
+//   16-bit weights, six: bfloat16 gradients 956 -> 948 us, float32 ones 1035 -> 1025 (odd sizes 184 -> 187, 204 -> 202)
+//   float32 weights alone, none: float32 gradients 1286 -> 1283 us with six and 1304 with five; bfloat16 ones 1143 -> 1122 with
+//     six, but 140 -> 145 at 2^25 values.
+// The other kernels gain nothing.
 template <class PT, class LT>
 constexpr unsigned idle_lds() {
   return !__is_same(LT, None) ? 160 * 1024 / 5 : sizeof(PT) == 2 ? 160 * 1024 / 6 / 512 * 512 : 0;
