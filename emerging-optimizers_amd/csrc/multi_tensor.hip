@@ -278,7 +278,8 @@ __global__ __launch_bounds__(NT) void adamw_kernel(AdamArgs<LT> a) {
 //   u = fraction of (t c + i a)   for step t and place i of the tensor, c and a irrational, others for v than for m.
 // For each place u rotates through its interval evenly, so a change of 0.01 of a code moves it every 100 steps, and the
 // errors of consecutive steps cancel instead of adding up as independent random numbers' do.  Two rules beside it: codes of
-// v below 6 round up (a root of v held at a fraction of itself blows the update up), and the first four steps go to nearest
+// v below 6 round up (a root of v held at a fraction of itself blows the update up; so a root that falls stops at
+// 1/1800 of its block's largest, which makes such a value's updates smaller, never larger), and the first four steps go to nearest
 // (step t of a moving average changes a code by about 1 / (2 t) of itself, so nothing stands still yet).
 // Simulated update error against 32-bit moments, gradients' scales spread as exp(N(0, sigma)), beta2 = 0.95 / 0.999:
 //   sigma 0.5: nearest 2.3 / 5.6 %, independent random numbers 3.3 / 6.9 %, rotating 2.5 / 5.8 %

@@ -102,7 +102,8 @@ def fused_adamw_update_8bit(
     updates.  Over a run of steps it stops a moving average whose step is less than half the distance between two codes: with
     ``beta2=0.999`` a second moment whose gradients shrink never follows them while the largest one of its block stays.
     "dithered" is for training loops: from the fifth step on the code is the next one below or above, by an offset that rotates
-    with ``step`` (see ``mi_adamw_update``), so moments follow on average; consecutive calls need consecutive ``step``.
+    with ``step`` (see ``mi_adamw_update``), so moments follow on average (the root of a second one down to 1/1800 of its
+    block's largest); consecutive calls need consecutive ``step``.
     """
     bits = _ROUNDING_BITS.get(rounding)
     if bits is None:

@@ -252,6 +252,7 @@ int mi_muon_update_bf16(float* param, const float* grad, float* momentum, int64_
  *   |k| = floor(y + u), y = 127 sqrt(|m| / s) or 255 (v / s)^(1/4), at most 127 or 255,
  *   u = ((t * c + i * a) mod 2^32 >> 9) / 2^23 for place i of the tensor (in memory order) and the whole part of t,
  *   c, a = 0x9E3779B9, 0x6A09E667 for m and 0x6A09E667, 0xBB67AE85 for v; u = 255/256 for y < 6 in v; u = 1/2 for t <= 4.
+ * (So a second moment that falls stops at (6/255)^4 of its block's largest.)
  * Consecutive steps have to have consecutive t; the same call gives the same codes.
  * (With 8-bit moments a second moment below 2^-126 counts as 0, in the update too.)
  * t = step (>= 1), or, where step_dev is not NULL, *step_dev[i] for tensor i (float32 on the device).
